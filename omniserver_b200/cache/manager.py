@@ -11,6 +11,8 @@ Here a request holds only the pages its tokens need:
 * Pages are taken when a step brings tokens (``reserve``), given back when a request ends, and,
   in a group with a window, as soon as every position of the page is older than any future query
   can see (``commit``).  A freed page is the next one handed out.
+* A request can be forked (``fork``): the full pages of the prefix then have two holders, and only the partly filled
+  last page is copied.  Tokens are written at a request's cursor and behind it, so a page with two holders is never written.
 * Storage per group: ``[layers, 2, pages, kv_heads, page_size, head_dim]`` (keys, values).
 """
 
@@ -22,6 +24,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from .. import ops
 from ..parts.base import CacheBinding, KVCacheNeed, StateNeed
 from .page_pool import OutOfPages, PagePool
 from .state_slots import OutOfSlots, StateSlots
@@ -183,6 +186,39 @@ class CacheManager:
         self.requests[request_id] = rc
         return rc
 
+    def fork(self, parent_id: str, child_id: str) -> RequestCache:
+        """A new request with the parent's tokens in its cache, between two steps: it shares the parent's full pages, gets a copy
+        of the partly filled one, and a slot with a copy of the parent's state. All or nothing."""
+        parent = self.requests[parent_id]
+        if parent.reserved:
+            raise ValueError(f"request {parent_id!r} cannot be forked while a step of it runs")
+        partial = parent.cursor // self.page_size if parent.cursor % self.page_size else None
+        copies = [partial is not None and t[partial] >= 0 for t in parent.tables]
+        for copy, g in zip(copies, self.groups):
+            if copy and g.pool.num_free < 1:
+                raise OutOfPages(f"request {child_id!r} needs a page, none is free")
+        child = self.begin(child_id)
+        try:
+            for gi, (copy, g) in enumerate(zip(copies, self.groups)):
+                for pi, page in enumerate(parent.tables[gi]):
+                    if copy and pi == partial:
+                        mine = g.pool.alloc()
+                        child.tables[gi].append(mine)
+                        if g.storage is not None:
+                            ops.kernels().copy_pages(g.storage, [page], [mine])
+                    else:
+                        if page >= 0:
+                            g.pool.share(page)
+                        child.tables[gi].append(page)
+                child.first_live[gi] = parent.first_live[gi]
+            for t in self.state.tensors.values():
+                t[child.slot].copy_(t[parent.slot])
+        except Exception:
+            self.finish(child_id)
+            raise
+        child.cursor = parent.cursor
+        return child
+
     def has(self, request_id: str) -> bool:
         return request_id in self.requests
 
@@ -251,6 +287,12 @@ class CacheManager:
                 rc.tables[gi][pi] = -1
             rc.first_live[gi] = max(rc.first_live[gi], first)
 
+    def accept(self, request_id: str, n_kept: int) -> None:
+        """A step of drafted tokens was verified: the first ``n_kept`` of the reserved tokens (where ``compact_cache`` puts the
+        accepted ones) are in the cache, the pages that only the others needed go back to the pool."""
+        self.commit(request_id, n_kept)
+        self.rollback(request_id)
+
     def rollback(self, request_id: str) -> None:
         """Undoes the reservations of a step that did not run: the pages taken beyond the request's cursor go
         back to the pool and nothing stays reserved."""
@@ -267,7 +309,7 @@ class CacheManager:
     def _release(self, g: PageGroup, page: int) -> None:
         if page < 0:
             return
-        if self.poison_freed and g.storage is not None:
+        if self.poison_freed and g.storage is not None and g.pool.holders(page) == 1:
             g.storage[:, :, page] = float("nan")
         g.pool.free(page)
 
@@ -339,17 +381,18 @@ class CacheManager:
         return [g.pool.num_free for g in self.groups]
 
     def check_invariants(self) -> None:
-        """No page lost, none held twice: every held page is in exactly one live table."""
+        """No page lost, none held by more block tables than it has holders (one, unless a request was forked)."""
         for gi, g in enumerate(self.groups):
-            seen = set()
+            seen: Dict[int, int] = {}
             for rc in self.requests.values():
                 for p in rc.tables[gi]:
                     if p < 0:
                         continue
-                    if p in seen:
-                        raise AssertionError(f"group {gi}: page {p} is in two block tables")
+                    seen[p] = seen.get(p, 0) + 1
                     if not g.pool.is_held(p):
                         raise AssertionError(f"group {gi}: page {p} is in a block table but free")
-                    seen.add(p)
+            for p, n in seen.items():
+                if n != g.pool.holders(p):
+                    raise AssertionError(f"group {gi}: page {p} is in {n} block tables and has {g.pool.holders(p)} holders")
             if len(seen) != g.pool.num_held:
                 raise AssertionError(f"group {gi}: {g.pool.num_held} pages held, {len(seen)} in block tables")

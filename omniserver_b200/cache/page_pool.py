@@ -11,14 +11,15 @@ class OutOfPages(RuntimeError):
 
 class PagePool:
     """Hands out page ids 0..num_pages-1. Last freed, first reused, so that pages are used again
-    soon (a stale read then shows up in tests instead of hiding in never-touched memory)."""
+    soon (a stale read then shows up in tests instead of hiding in never-touched memory).
+    A page may have several holders (``share``: forked requests); it is free when the last one gives it back."""
 
     def __init__(self, num_pages: int):
         if num_pages <= 0:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = int(num_pages)
         self._free: List[int] = list(range(self.num_pages - 1, -1, -1))
-        self._held = [False] * self.num_pages
+        self._holders = [0] * self.num_pages
 
     @property
     def num_free(self) -> int:
@@ -32,16 +33,26 @@ class PagePool:
         if not self._free:
             raise OutOfPages("no free page")
         p = self._free.pop()
-        self._held[p] = True
+        self._holders[p] = 1
         return p
+
+    def share(self, page: int) -> None:
+        """One more holder of a page that is held."""
+        if not (0 <= page < self.num_pages) or self._holders[page] == 0:
+            raise ValueError(f"page {page} is not held by anyone")
+        self._holders[page] += 1
 
     def free(self, page: int) -> None:
         if not (0 <= page < self.num_pages):
             raise ValueError(f"page {page} is not of this pool")
-        if not self._held[page]:
+        if self._holders[page] == 0:
             raise ValueError(f"page {page} freed twice (or never handed out)")
-        self._held[page] = False
-        self._free.append(page)
+        self._holders[page] -= 1
+        if self._holders[page] == 0:
+            self._free.append(page)
+
+    def holders(self, page: int) -> int:
+        return self._holders[page]
 
     def is_held(self, page: int) -> bool:
-        return self._held[page]
+        return self._holders[page] > 0

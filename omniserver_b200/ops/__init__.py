@@ -25,9 +25,10 @@ from .library import KernelLibraryError
 
 from ._common import _DEVICE_ERR, _STATUS, KernelError, _check, _cuda_contig, _dt, _p
 from .persistent import PersistentDecodeOps
+from .speculative import SpeculativeOps
 
 
-class CudaKernels(PersistentDecodeOps):
+class CudaKernels(PersistentDecodeOps, SpeculativeOps):
     """Launches the hand-written kernels. One instance per process."""
 
     #: rows up to which the bf16 weight-streaming GEMM is used instead of the tiled tensor-core GEMM

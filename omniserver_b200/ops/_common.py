@@ -26,6 +26,9 @@ _DEVICE_ERR = {
     2: "an embedding-override row outside the step's tokens",
     3: "a cache slot outside the page pool in the key/value write",
     4: "a page index outside the page pool in attention",
+    5: "a drafted token outside the vocabulary reached the verification",
+    6: "a path that does not ascend within its tree reached the cache compaction",
+    7: "a request has more nodes or keys than the call to the tree attention allowed for",
     101: "tcgen05 GEMM: the TMA producer waited too long for a free stage",
     102: "tcgen05 GEMM: the MMA issuer waited too long for operands",
     103: "tcgen05 GEMM: the epilogue waited too long for the accumulator",
