@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(
   if (split >= n_splits) return;
   const int k_begin = split * chunk, k_end = min(kv_len, k_begin + chunk);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  if ((kv_all > kv_len || n > max_q_len) && split == 0 && tid == 0) atomicExch(err, ERR_BOUNDS);
+  if ((kv_all > kv_len || n > max_q_len || base < 0) && split == 0 && tid == 0) atomicExch(err, ERR_BOUNDS);
 
   const bool vec = (hd & 3) == 0 && ((q_row_stride & 3) == 0) &&
                    (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0;
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(
     const int r = r0 + ty * ROWS + i;
     node_of[i] = r < rows ? r / grp : -1;
     lo_of[i] = 0;
-    if (window > 0 && node_of[i] >= 0) lo_of[i] = base + depth[q0 + node_of[i]] - window + 1;
+    if (window > 0 && node_of[i] >= 0) lo_of[i] = base + min(max(depth[q0 + node_of[i]], 0), n - 1) - window + 1;
     m[i] = -INFINITY;
     l[i] = 0.0f;
 #pragma unroll
@@ -274,7 +274,7 @@ OSB_API int osb_attn_tree_splits(int max_kv_len) {
 }
 
 // out [T, nh*hd]; q rows of q_row_stride elements, caches [num_pages, nkv, page_size, hd], mask [T, mask_words] words, depth [T]
-// (needed with a window). part_o [T*nh*splits*hd], part_ml [T*nh*splits*2] floats with splits = osb_attn_tree_splits(max_kv_len) > 1.
+// (needed with a window; below the request's number of nodes). part_o [T*nh*splits*hd], part_ml [T*nh*splits*2] floats with splits = osb_attn_tree_splits(max_kv_len) > 1.
 // max_q_len / max_kv_len: at least the largest of the batch; a request beyond them is reported in *err, and what lies beyond is
 // not computed.
 OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, int q_row_stride, const void* k_cache,

@@ -108,6 +108,25 @@ class SpeculativeOps:
         if S == 0 or T == 0 or max_q_len <= 0 or max_kv_len <= 0 or k_cache.shape[0] == 0:
             return out
         part_o = part_ml = None
+        splits = 0
+        if (not exact and qkv.dtype == k_cache.dtype == out_dtype == torch.bfloat16
+                and (qkv.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0):
+            splits = self.lib.osb_attn_tree_tc_splits(S, nh, nkv, hd, k_cache.shape[2], qkv.shape[1], ctypes.c_float(scale), win,
+                                                      max_q_len, max_kv_len)
+        if splits > 0:
+            if splits > 1:
+                nodes = 128 // (nh // nkv)
+                rows = S * nkv * -(-max_q_len // nodes) * splits * 128
+                part_o = torch.empty(rows * hd, dtype=torch.float32, device=qkv.device)
+                part_ml = torch.empty(rows * 2, dtype=torch.float32, device=qkv.device)
+            rc = self.lib.osb_attn_tree_tc(
+                _p(out), _p(qkv), qkv.shape[1], T, _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(cu_q),
+                _p(seq_lens), _p(tree_mask), tree_mask.shape[1], _p(depth), S, nh, nkv, hd, k_cache.shape[2], k_cache.shape[0],
+                ctypes.c_float(scale), win, max_q_len, max_kv_len, splits, _p(part_o), _p(part_ml),
+                _p(self.err_flag(qkv.device)), self._stream())
+            self._ok(rc, "attn_tree_tc")
+            self.launches += 1 if splits > 1 else 0
+            return out
         splits = self.lib.osb_attn_tree_splits(max_kv_len)
         if splits > 1:
             part_o = torch.empty(T * nh * splits * hd, dtype=torch.float32, device=qkv.device)

@@ -115,7 +115,10 @@ BATCHES = [
 @pytest.mark.parametrize("q_lens,bases", BATCHES)
 def test_tree_attention(q_lens, bases, nh, nkv, hd, dtype):
     step = Step(q_lens, bases, nh, nkv, hd, 16, dtype, seed=len(q_lens) + hd)
-    check(step, step.got(), *step.want(), runs_on_tensor_cores(step))
+    before = K().counts["attn_tree_tc"]
+    got = step.got()
+    assert K().counts["attn_tree_tc"] - before == (1 if runs_on_tensor_cores(step) else 0)
+    check(step, got, *step.want(), runs_on_tensor_cores(step))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
