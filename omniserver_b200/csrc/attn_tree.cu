@@ -300,16 +300,16 @@ OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, 
         typedef OSB_T(ot) OT;
         const int hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
         const size_t smem = sizeof(float) * ((size_t)(RT + 2 * KT) * (hdp + 4) + RT * (KT + 4));
-        auto go = [&](auto k) -> int {
-          const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-          if (e != cudaSuccess) return (int)e;
+        auto go = [&](auto k, int rc) -> int {
+          if (rc) return rc;
           return osb_launch(k, dim3((unsigned)(tiles * splits), (unsigned)nkv, (unsigned)S), dim3(NT), smem, stream, (OT*)out,
                             part_o, part_ml, (const QT*)q, q_row_stride, (const KVT*)k_cache, (const KVT*)v_cache, block_table,
                             bt_stride, cu_q, seq_lens, mask, mask_words, depth, nh, nkv, hd, page_size, num_pages, scale,
                             window, splits, max_q_len, kv_cap, err);
         };
-        int rc = hdp == 64 ? go(attn_tree_kernel<QT, KVT, OT, 64>)
-                           : hdp == 128 ? go(attn_tree_kernel<QT, KVT, OT, 128>) : go(attn_tree_kernel<QT, KVT, OT, 256>);
+        int rc = hdp == 64    ? go(attn_tree_kernel<QT, KVT, OT, 64>, osb_allow_smem<attn_tree_kernel<QT, KVT, OT, 64>>(smem))
+                 : hdp == 128 ? go(attn_tree_kernel<QT, KVT, OT, 128>, osb_allow_smem<attn_tree_kernel<QT, KVT, OT, 128>>(smem))
+                              : go(attn_tree_kernel<QT, KVT, OT, 256>, osb_allow_smem<attn_tree_kernel<QT, KVT, OT, 256>>(smem));
         if (rc) return rc;
         if (splits > 1) {
           const long long blocks = ((long long)max_q_len * nh + 3) / 4;

@@ -681,12 +681,6 @@ __global__ void __launch_bounds__(BLOCK_M) attn_tree_tc_join_kernel(bf16* __rest
   *reinterpret_cast<uint4*>(out + ((size_t)(q0 + node0 + node) * plan.nh + kvh * plan.grp + g) * HD + d8 * 8) = w;
 }
 
-int num_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
-  return n > 0 ? n : 1;
-}
-
 // Key tiles that a request of the batch looks at, at most.
 int most_tiles(int max_q_len, int max_kv_len, int window) {
   long long t = ((long long)max_kv_len + TILE_N - 1) / TILE_N;
@@ -703,11 +697,11 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   // at least 120 KB so that one CTA is resident per SM: each takes all 512 tensor-memory columns
   constexpr size_t need = (size_t)(HD / 64) * ATOM_BYTES * (1 + 2 * STAGES) + 1024;
   constexpr size_t smem = need > 120 * 1024 ? need : 120 * 1024;
-  auto k = attn_tree_tc_kernel<HD>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
-  const int sms = num_sms();
-  int rc = osb_launch(k, dim3((unsigned)(plan.n_items < sms ? plan.n_items : sms)), dim3(NUM_THREADS), smem, stream, mq, mk, mv, out,
+  int sms = 0;
+  int rc = osb_allow_smem<attn_tree_tc_kernel<HD>>(smem);
+  if (rc == 0) rc = osb_num_sms(&sms);
+  if (rc) return rc;
+  rc = osb_launch(attn_tree_tc_kernel<HD>, dim3((unsigned)(plan.n_items < sms ? plan.n_items : sms)), dim3(NUM_THREADS), smem, stream, mq, mk, mv, out,
                       (float4*)part_o, (float2*)part_ml, v_cache, plan, scale_log2, err);
   if (rc == 0 && plan.splits > 1)
     rc = osb_launch(attn_tree_tc_join_kernel<HD>, dim3((unsigned)(plan.S * plan.nkv * plan.m_tiles), HD / 8), dim3(BLOCK_M), 0, stream,
@@ -727,7 +721,9 @@ OSB_API int osb_attn_tree_tc_splits(int S, int nh, int nkv, int hd, int page_siz
   const int nodes = BLOCK_M / (nh / nkv);
   const long long units = (long long)S * nkv * ((max_q_len + nodes - 1) / nodes);
   if (units * MAX_TC_SPLITS > 2147483647LL) return 0;
-  const int tiles = most_tiles(max_q_len, max_kv_len, window), sms = num_sms();
+  const int tiles = most_tiles(max_q_len, max_kv_len, window);
+  int sms = 1;
+  osb_num_sms(&sms);
   int best = 1;
   long long best_cost = 0;
   for (int s = 1; s <= MAX_TC_SPLITS && s <= tiles; ++s) {

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #define OSB_API extern "C" __attribute__((visibility("default")))
@@ -69,6 +70,35 @@ __device__ __forceinline__ float block_max(float v, float* smem32) {
 }
 
 static inline int osb_last_error() { return (int)cudaGetLastError(); }
+
+// What a launch asks about the current device, asked once per device.
+constexpr int OSB_MAX_DEVICES = 64;
+static inline int osb_num_sms(int* out) {
+  static std::atomic<int> known[OSB_MAX_DEVICES];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  int n = dev < OSB_MAX_DEVICES ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < OSB_MAX_DEVICES) known[dev].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return 0;
+}
+template <auto Kernel> static inline int osb_allow_smem(size_t bytes) {
+  static std::atomic<int> allowed[OSB_MAX_DEVICES];
+  if (bytes <= 48 * 1024) return 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev < OSB_MAX_DEVICES && allowed[dev].load(std::memory_order_relaxed) >= (int)bytes) return 0;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return (int)e;
+  if (dev < OSB_MAX_DEVICES) allowed[dev].store((int)bytes, std::memory_order_relaxed);
+  return 0;
+}
 
 // Programmatic dependent launch: a kernel launched through osb_launch may start while the kernel
 // before it in the stream is finishing; it must call pdl_wait() before it reads or writes anything

@@ -14,25 +14,72 @@ The reference has none of these (it decodes one token per request and step, omni
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence, Tuple
+from operator import index
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
-from ._common import _check, _cuda_contig, _dt, _p
+from ._common import KernelError, _check, _cuda_contig, _dt
+
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+
+_PTR, _INT, _FLOAT, _LONG = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
+_SIGNATURES = {
+    "osb_attn_tree_splits": [_INT],
+    "osb_attn_tree": [_PTR, _INT, _PTR, _INT, _INT, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT,
+                      _INT, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR],
+    "osb_attn_tree_tc_splits": [_INT, _INT, _INT, _INT, _INT, _INT, _FLOAT, _INT, _INT, _INT],
+    "osb_attn_tree_tc": [_PTR, _PTR, _INT, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT, _INT, _INT,
+                         _FLOAT, _INT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR],
+    "osb_verify_drafts": [_PTR] * 11 + [_INT] * 5 + [_PTR, _PTR],
+    "osb_compact_cache": [_PTR, _INT, _INT, _INT, _INT, _INT, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR],
+    "osb_copy_pages": [_PTR, _LONG, _INT, _INT, _PTR, _PTR, _INT, _PTR],
+}
 
 
-def _on_device(ref: torch.Tensor, **tensors: Optional[torch.Tensor]) -> None:
-    """Every tensor on the current device: a launch goes to a stream of that one."""
-    dev = ref.device
-    _check(dev.index == torch.cuda.current_device(), f"the tensors are on {dev}, which is not the current device")
+def declare(lib: ctypes.CDLL) -> None:
+    """The argument types of this file's entry points, so that plain integers can be handed over as addresses: these calls are made
+    where a step's launches take a few microseconds, and an object per address costs about as much."""
+    for name, types in _SIGNATURES.items():
+        getattr(lib, name).argtypes = types
+
+
+def _on_device(ref: torch.Tensor) -> int:
+    """The index of the tensor's device, which has to be the current one: a launch goes to a stream of that."""
+    _check(ref.is_cuda, "the operands must be CUDA tensors (there is no CPU path)")
+    dev = ref.get_device()
+    if dev != torch.cuda.current_device():
+        raise KernelError(f"the tensors are on cuda:{dev}, which is not the current device")
+    return dev
+
+
+def _operands(dev: int, dtype: Optional[torch.dtype], **tensors: torch.Tensor) -> None:
+    """Contiguous tensors of this type on this device."""
     for name, t in tensors.items():
-        _check(t is None or t.device == dev, f"{name} must be on {dev}")
+        if t.get_device() != dev or (dtype is not None and t.dtype is not dtype) or not t.is_contiguous():
+            _cuda_contig(name, t, dtype)
+            raise KernelError(f"{name} must be on cuda:{dev}")
+
+
+def _page_numbers(pages: Sequence[int]) -> List[int]:
+    """The numbers as a list; anything but a row of whole numbers on the host is refused."""
+    try:
+        return [index(p) for p in (pages if isinstance(pages, (list, tuple)) else np.asarray(pages))]
+    except TypeError as e:
+        raise KernelError(f"copy_pages: page numbers are whole numbers on the host: {e}") from None
 
 
 class SpeculativeOps:
     MAX_TREE_NODES = 1024      # of one request, in ``verify_drafts``
-    VERIFY_SLICE = 4096        # words of a logits row that one CTA of the verification takes
+    VERIFY_SLICE = 1024        # words of a logits row that a warp of the verification takes at a time
+
+    def _raw_stream(self, dev: int) -> int:
+        """The current stream of device ``dev`` (the pinned one inside ``pinned_stream``) as an address. Looking up
+        ``torch.cuda.current_stream()`` makes a Stream object, 3.4 us of the 14 that a small call takes on the host."""
+        if self._pinned_stream is not None:
+            return self._pinned_stream.value or 0
+        return torch._C._cuda_getCurrentRawStream(dev)
 
     # ------------------------------------------------------------------ plan of a step (host)
     @staticmethod
@@ -76,67 +123,69 @@ class SpeculativeOps:
         Rows of ``out`` [T, nh*hd] (made here if not given) that belong to no request are not written. float32 operands,
         ``exact=True`` and shapes the tensor-core kernel does not take run in 32 bits throughout.
         """
-        _cuda_contig("qkv", qkv)
-        _cuda_contig("k_cache", k_cache)
-        _cuda_contig("v_cache", v_cache)
-        for n, t in (("block_table", block_table), ("cu_q", cu_q), ("seq_lens", seq_lens), ("tree_mask", tree_mask)):
-            _cuda_contig(n, t, torch.int32)
+        dev = _on_device(qkv)
+        _operands(dev, None, qkv=qkv, k_cache=k_cache, v_cache=v_cache)
+        _operands(dev, _I32, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, tree_mask=tree_mask)
         win = int(window) if window else 0
         _check(win >= 0, "tree_attention: a window is positive")
-        _check(win == 0 or depth is not None, "tree_attention: a window needs the nodes' depth")
-        if depth is not None:
-            _cuda_contig("depth", depth, torch.int32)
-        _on_device(qkv, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens,
-                   tree_mask=tree_mask, depth=depth, out=out)
-        _check(qkv.dim() == 2 and seq_lens.dim() == 1, "tree_attention: qkv [T,*], seq_lens [S]")
-        T, S = qkv.shape[0], seq_lens.shape[0]
+        _check(qkv.dim() == 2 and seq_lens.dim() == 1 and block_table.dim() == 2 and tree_mask.dim() == 2 and k_cache.dim() == 4,
+               "tree_attention: qkv [T,*], seq_lens [S], block_table [S,*], tree_mask [T,W], caches [pages, nkv, page_size, hd]")
+        T, width = qkv.shape
+        S, = seq_lens.shape
+        pages, heads, page_size, head_dim = shape = k_cache.shape
+        rows, words = tree_mask.shape
+        tables, bt_width = block_table.shape
         _check(nh > 0 and nkv > 0 and hd > 0 and nh % nkv == 0, "tree_attention: heads must be a multiple of kv heads")
-        _check(qkv.shape[1] >= nh * hd, "tree_attention: q columns missing")
-        _check(k_cache.dim() == 4 and k_cache.shape[1] == nkv and k_cache.shape[3] == hd and v_cache.shape == k_cache.shape
-               and v_cache.dtype == k_cache.dtype, "tree_attention: caches [pages, nkv, page_size, hd]")
-        _check(block_table.dim() == 2 and block_table.shape[0] == S, "tree_attention: block_table [S,*]")
+        _check(width >= nh * hd, "tree_attention: q columns missing")
+        _check(heads == nkv and head_dim == hd and v_cache.shape == shape and v_cache.dtype is k_cache.dtype,
+               "tree_attention: caches [pages, nkv, page_size, hd]")
+        _check(tables == S, "tree_attention: block_table [S,*]")
         _check(cu_q.shape == (S + 1,), "tree_attention: cu_q [S+1]")
-        _check(tree_mask.dim() == 2 and tree_mask.shape[0] == T and 32 * tree_mask.shape[1] >= max_q_len,
-               "tree_attention: tree_mask [T, W] with 32 W >= max_q_len")
-        _check(depth is None or depth.shape == (T,), "tree_attention: depth [T]")
+        _check(rows == T and 32 * words >= max_q_len, "tree_attention: tree_mask [T, W] with 32 W >= max_q_len")
         _check(hd <= 256, "tree_attention: head sizes up to 256")
+        if depth is not None:
+            _operands(dev, _I32, depth=depth)
+            _check(depth.shape == (T,), "tree_attention: depth [T]")
+        else:
+            _check(win == 0, "tree_attention: a window needs the nodes' depth")
         if out is None:
             out = torch.empty((T, nh * hd), dtype=out_dtype, device=qkv.device)
         else:
-            _cuda_contig("out", out, out_dtype)
+            _operands(dev, out_dtype, out=out)
             _check(out.shape == (T, nh * hd), "tree_attention: out [T, nh*hd]")
-        if S == 0 or T == 0 or max_q_len <= 0 or max_kv_len <= 0 or k_cache.shape[0] == 0:
+        if S == 0 or T == 0 or max_q_len <= 0 or max_kv_len <= 0 or pages == 0:
             return out
-        part_o = part_ml = None
+        qp, kp, vp, op = qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+        dp = depth.data_ptr() if depth is not None else None
+        err = self.err_flag(qkv.device).data_ptr()
         splits = 0
-        if (not exact and qkv.dtype == k_cache.dtype == out_dtype == torch.bfloat16
-                and (qkv.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr() | out.data_ptr()) % 16 == 0):
-            splits = self.lib.osb_attn_tree_tc_splits(S, nh, nkv, hd, k_cache.shape[2], qkv.shape[1], ctypes.c_float(scale), win,
-                                                      max_q_len, max_kv_len)
+        if (not exact and qkv.dtype is _BF16 and k_cache.dtype is _BF16 and out_dtype is _BF16 and (qp | kp | vp | op) % 16 == 0):
+            splits = self.lib.osb_attn_tree_tc_splits(S, nh, nkv, hd, page_size, width, scale, win, max_q_len, max_kv_len)
         if splits > 0:
+            # rows of a row tile's ranges, then (maximum, sum) of each
+            part = ml = None
             if splits > 1:
-                nodes = 128 // (nh // nkv)
-                rows = S * nkv * -(-max_q_len // nodes) * splits * 128
-                part_o = torch.empty(rows * hd, dtype=torch.float32, device=qkv.device)
-                part_ml = torch.empty(rows * 2, dtype=torch.float32, device=qkv.device)
+                slots = S * nkv * -(-max_q_len // (128 // (nh // nkv))) * splits * 128
+                scratch = torch.empty(slots * (hd + 2), dtype=_F32, device=qkv.device)
+                part = scratch.data_ptr()
+                ml = part + 4 * slots * hd
             rc = self.lib.osb_attn_tree_tc(
-                _p(out), _p(qkv), qkv.shape[1], T, _p(k_cache), _p(v_cache), _p(block_table), block_table.shape[1], _p(cu_q),
-                _p(seq_lens), _p(tree_mask), tree_mask.shape[1], _p(depth), S, nh, nkv, hd, k_cache.shape[2], k_cache.shape[0],
-                ctypes.c_float(scale), win, max_q_len, max_kv_len, splits, _p(part_o), _p(part_ml),
-                _p(self.err_flag(qkv.device)), self._stream())
+                op, qp, width, T, kp, vp, block_table.data_ptr(), bt_width, cu_q.data_ptr(), seq_lens.data_ptr(),
+                tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len, max_kv_len, splits, part,
+                ml, err, self._raw_stream(dev))
             self._ok(rc, "attn_tree_tc")
-            self.launches += 1 if splits > 1 else 0
-            return out
-        splits = self.lib.osb_attn_tree_splits(max_kv_len)
-        if splits > 1:
-            part_o = torch.empty(T * nh * splits * hd, dtype=torch.float32, device=qkv.device)
-            part_ml = torch.empty(T * nh * splits * 2, dtype=torch.float32, device=qkv.device)
-        rc = self.lib.osb_attn_tree(
-            _p(out), _dt(out), _p(qkv), _dt(qkv), qkv.shape[1], _p(k_cache), _p(v_cache), _dt(k_cache), _p(block_table),
-            block_table.shape[1], _p(cu_q), _p(seq_lens), _p(tree_mask), tree_mask.shape[1], _p(depth), S, nh, nkv, hd,
-            k_cache.shape[2], k_cache.shape[0], ctypes.c_float(scale), win, max_q_len, max_kv_len, _p(part_o), _p(part_ml),
-            _p(self.err_flag(qkv.device)), self._stream())
-        self._ok(rc, "attn_tree")
+        else:
+            splits = self.lib.osb_attn_tree_splits(max_kv_len)
+            part = ml = None
+            if splits > 1:
+                scratch = torch.empty(T * nh * splits * (hd + 2), dtype=_F32, device=qkv.device)
+                part = scratch.data_ptr()
+                ml = part + 4 * T * nh * splits * hd
+            rc = self.lib.osb_attn_tree(
+                op, _dt(out), qp, _dt(qkv), width, kp, vp, _dt(k_cache), block_table.data_ptr(), bt_width, cu_q.data_ptr(),
+                seq_lens.data_ptr(), tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len,
+                max_kv_len, part, ml, err, self._raw_stream(dev))
+            self._ok(rc, "attn_tree")
         self.launches += 1 if splits > 1 else 0
         return out
 
@@ -159,45 +208,51 @@ class SpeculativeOps:
         drafted tokens are accepted. A request without nodes has count 0. A token outside the vocabulary is never accepted, and
         reported by ``check_device_errors`` where a request brings it as a draft.
         """
-        _cuda_contig("logits", logits, torch.float32)
-        for n, t in (("tokens", tokens), ("parents", parents), ("cu_q", cu_q)):
-            _cuda_contig(n, t, torch.int32)
-        _cuda_contig("uniform", uniform, torch.float32)
+        dev = _on_device(logits)
+        _operands(dev, _F32, logits=logits, uniform=uniform)
+        _operands(dev, _I32, tokens=tokens, parents=parents, cu_q=cu_q)
         _check(logits.dim() == 2 and cu_q.dim() == 1 and cu_q.shape[0] >= 1, "verify_drafts: logits [T,V], cu_q [S+1]")
         T, V = logits.shape
         S = cu_q.shape[0] - 1
         _check(V > 0, "verify_drafts: an empty vocabulary")
         _check(tokens.shape == (T,) and parents.shape == (T,) and uniform.shape == (T,),
                "verify_drafts: tokens, parents and uniform [T]")
-        _check(0 <= max_q_len <= self.MAX_TREE_NODES, f"verify_drafts: up to {self.MAX_TREE_NODES} nodes per request")
+        _check(0 <= max_q_len <= self.MAX_TREE_NODES, "verify_drafts: up to 1024 nodes per request")
         _check(max_depth >= 0, "verify_drafts: max_depth must not be negative")
+        tp = qp = None
         if temperature is not None:
-            _cuda_contig("temperature", temperature, torch.float32)
+            _operands(dev, _F32, temperature=temperature)
             _check(temperature.shape == (S,), "verify_drafts: temperature [S]")
+            tp = temperature.data_ptr()
         if draft_probs is not None:
-            _cuda_contig("draft_probs", draft_probs, torch.float32)
+            _operands(dev, _F32, draft_probs=draft_probs)
             _check(draft_probs.shape == (T, V), "verify_drafts: draft_probs [T,V]")
-        _on_device(logits, tokens=tokens, parents=parents, cu_q=cu_q, uniform=uniform, temperature=temperature,
-                   draft_probs=draft_probs)
-        out = torch.empty((2 * (max_depth + 1) + 1) * S, dtype=torch.int32, device=logits.device)
-        n = S * (max_depth + 1)
-        new, path, count = out[:n].view(S, max_depth + 1), out[n:2 * n].view(S, max_depth + 1), out[2 * n:]
+            qp = draft_probs.data_ptr()
+        # the three results, and behind them, on a 16-byte boundary, 16 bytes per slice of a row for the kernels
+        w = max_depth + 1
+        n = S * w
+        head = (2 * n + S + 3) & ~3
+        buf = torch.empty(head + 4 * T * -(-V // self.VERIFY_SLICE), dtype=_I32, device=logits.device)
+        new, path, count = buf[:n].view(S, w), buf[n:2 * n].view(S, w), buf[2 * n:2 * n + S]
         if S == 0:
             return new, path, count
-        stats = torch.empty(max(1, T) * -(-V // self.VERIFY_SLICE) * 2, dtype=torch.float64, device=logits.device)
-        rc = self.lib.osb_verify_drafts(_p(new), _p(path), _p(count), _p(stats), _p(logits), _p(tokens), _p(parents), _p(cu_q),
-                                        _p(uniform), _p(temperature), _p(draft_probs), S, T, V, max_q_len, max_depth,
-                                        _p(self.err_flag(logits.device)), self._stream())
+        at = buf.data_ptr()
+        rc = self.lib.osb_verify_drafts(at, at + 4 * n, at + 8 * n, at + 4 * head, logits.data_ptr(), tokens.data_ptr(),
+                                        parents.data_ptr(), cu_q.data_ptr(), uniform.data_ptr(), tp, qp, S, T, V, max_q_len,
+                                        max_depth, self.err_flag(logits.device).data_ptr(), self._raw_stream(dev))
         self._ok(rc, "verify_drafts")
         self.launches += 1 if T > 0 else 0
         return new, path, count
 
     # ------------------------------------------------------------------ cache
     @staticmethod
-    def _check_storage(what: str, cache: torch.Tensor) -> None:
-        _cuda_contig("cache", cache)
-        _check(cache.dim() == 6 and cache.shape[1] == 2, f"{what}: cache [layers, 2, pages, nkv, page_size, hd]")
+    def _storage(cache: torch.Tensor) -> Tuple[int, Tuple[int, ...]]:
+        """(device index, shape) of a page group's storage."""
+        dev = _on_device(cache)
+        _operands(dev, None, cache=cache)
+        _check(cache.dim() == 6 and cache.shape[1] == 2, "cache must be [layers, 2, pages, nkv, page_size, hd]")
         _dt(cache)
+        return dev, cache.shape
 
     def compact_cache(self, cache: torch.Tensor, block_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor,
                       path: torch.Tensor, count: torch.Tensor) -> None:
@@ -207,40 +262,36 @@ class SpeculativeOps:
         ``path`` and ``count`` as ``verify_drafts`` returns them. A path that does not ascend, leaves its tree, or is longer than
         it moves nothing of its request, and a token in a page outside the pool stays; both are reported by
         ``check_device_errors``."""
-        self._check_storage("compact_cache", cache)
-        for n, t in (("block_table", block_table), ("cu_q", cu_q), ("seq_lens", seq_lens), ("path", path), ("count", count)):
-            _cuda_contig(n, t, torch.int32)
+        dev, (L, _, P, nkv, ps, hd) = self._storage(cache)
+        _operands(dev, _I32, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, path=path, count=count)
         S = seq_lens.shape[0]
-        _check(seq_lens.dim() == 1 and cu_q.shape == (S + 1,) and count.shape == (S,), "compact_cache: seq_lens, count [S], cu_q [S+1]")
+        _check(seq_lens.dim() == 1 and cu_q.shape == (S + 1,) and count.shape == (S,),
+               "compact_cache: seq_lens, count [S], cu_q [S+1]")
         _check(block_table.dim() == 2 and block_table.shape[0] == S, "compact_cache: block_table [S,*]")
         _check(path.dim() == 2 and path.shape[0] == S, "compact_cache: path [S,*]")
-        _on_device(cache, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, path=path, count=count)
         if S == 0 or cache.numel() == 0:
             return
-        L, _, P, nkv, ps, hd = cache.shape
-        rc = self.lib.osb_compact_cache(_p(cache), cache.element_size(), 2 * L, P, nkv, ps, hd, _p(block_table), block_table.shape[1],
-                                        _p(cu_q), _p(seq_lens), _p(path), path.shape[1], _p(count), S,
-                                        _p(self.err_flag(cache.device)), self._stream())
+        rc = self.lib.osb_compact_cache(cache.data_ptr(), cache.element_size(), 2 * L, P, nkv, ps, hd, block_table.data_ptr(),
+                                        block_table.shape[1], cu_q.data_ptr(), seq_lens.data_ptr(), path.data_ptr(),
+                                        path.shape[1], count.data_ptr(), S, self.err_flag(cache.device).data_ptr(), self._raw_stream(dev))
         self._ok(rc, "compact_cache")
 
     def copy_pages(self, cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
         """Copies page src[i] to page dst[i] in every layer, keys and values. ``cache`` as for ``compact_cache``; the page numbers
         are on the host (as the block tables are): every dst once, and none of them a src."""
-        self._check_storage("copy_pages", cache)
-        _on_device(cache)
-        a = np.ascontiguousarray(src, dtype=np.int32)
-        b = np.ascontiguousarray(dst, dtype=np.int32)
-        _check(a.ndim == 1 and a.shape == b.shape, "copy_pages: as many sources as destinations")
-        n = a.shape[0]
+        dev, (L, _, P, nkv, ps, hd) = self._storage(cache)
+        a, b = _page_numbers(src), _page_numbers(dst)
+        n = len(a)
+        _check(n == len(b), "copy_pages: as many sources as destinations")
         if n == 0:
             return
-        la, lb = a.tolist(), b.tolist()
-        L, _, P, nkv, ps, hd = cache.shape
-        _check(min(la) >= 0 and max(la) < P and min(lb) >= 0 and max(lb) < P, f"copy_pages: pages 0 to {P - 1}")
-        to = set(lb)
-        _check(len(to) == n and to.isdisjoint(la), "copy_pages: every destination once, and none of them a source")
+        _check(min(a) >= 0 and max(a) < P and min(b) >= 0 and max(b) < P, "copy_pages: a page outside the pool")
+        to = set(b)
+        _check(len(to) == n and to.isdisjoint(a), "copy_pages: every destination once, and none of them a source")
         if cache.numel() == 0:
             return
-        rc = self.lib.osb_copy_pages(_p(cache), ctypes.c_longlong(nkv * ps * hd * cache.element_size()), 2 * L, P,
-                                     ctypes.c_void_p(a.ctypes.data), ctypes.c_void_p(b.ctypes.data), n, self._stream())
+        pages = (ctypes.c_int * (2 * n))(*a, *b)
+        at = ctypes.addressof(pages)
+        rc = self.lib.osb_copy_pages(cache.data_ptr(), nkv * ps * hd * cache.element_size(), 2 * L, P, at, at + 4 * n, n,
+                                     self._raw_stream(dev))
         self._ok(rc, "copy_pages")

@@ -430,6 +430,32 @@ def test_verify_infinite_and_missing_logits(dense):
     assert got == want and all(x[0][0] == 0 and x[2] == 1 for x in got)
 
 
+@pytest.mark.parametrize("gaps", [(0.0, 1e-3), (0.0, 1e-7), (0.0, 0.1, 1e-4), (0.0, 1e-5, 1e-9), (0.0, 1e-12)])
+@pytest.mark.parametrize("together", [True, False])
+def test_verify_what_is_left_of_dominant_words(gaps, together):
+    """A few words hold nearly everything and are all rejected: what is left, down to 10^-12 of the row, keeps its digits."""
+    V, S = 30000, 24
+    g = torch.Generator().manual_seed(11)
+    words = [5000 + 3 * i if together else 700 + 5000 * i for i in range(len(gaps))]
+    rows = torch.randn(S, V, generator=g) * 2.0
+    rest = torch.logsumexp(rows.double(), -1)
+    for i, gap in enumerate(gaps):
+        nxt = gaps[i + 1] if i + 1 < len(gaps) else None
+        # word i outweighs everything behind it by 1 / (what is left next)
+        rows[:, words[i]] = (rest + sum(-math.log(x) for x in gaps[i + 1:]) if nxt else rest - 60).float()
+    n = len(gaps)
+    logits = torch.zeros(S * n, V)
+    logits[::n] = rows
+    tokens = i32(([0] + words[:n - 1]) * S)
+    u = torch.rand(S * n, generator=g)
+    u = (torch.floor(u * 2 ** 24) / 2 ** 24).float()
+    for k in range(1, n):
+        u[k::n] = 1.0 - 2.0 ** -24            # rejected wherever it can be
+    args = dict(logits=logits, tokens=tokens, parents=i32(([-1] + [0] * (n - 1)) * S), cu_q=i32(list(range(0, S * n + 1, n))), uniform=u)
+    got, want = verify_both(args, n, 1, torch.ones(S))
+    assert got == want
+
+
 def test_verify_equal_distributions_accept_everything():
     args, q = drafts([9], 4000, seed=6, branch=1, dense=True)
     q = torch.softmax(args["logits"].double(), -1)
@@ -626,9 +652,9 @@ def test_copy_pages_refuses():
     from omniserver_b200.ops import KernelError
     cache = paged([40], 2, 2, 8, 16, F32)[0].to(DEV)
     before = cache.clone()
-    for src, dst, match in [([0], [7], "pages 0 to 6"), ([-1], [1], "pages 0 to 6"), ([0, 1], [2, 2], "every destination once"),
+    for src, dst, match in [([0], [7], "outside the pool"), ([-1], [1], "outside the pool"), ([0.5], [1], "whole"), ([0, 1], [2, 2], "every destination once"),
                             ([0, 1], [1, 2], "none of them a source"), ([0], [0], "none of them a source"), ([0, 1], [2], "as many"),
-                            ([[0]], [[1]], "as many")]:
+                            ([[0]], [[1]], "whole"), (torch.tensor([0], device=DEV), [1], "whole")]:
         with pytest.raises(KernelError, match=match):
             K().copy_pages(cache, src, dst)
     with pytest.raises(KernelError, match="CUDA tensor"):
