@@ -1,24 +1,33 @@
 // Attention of a tree of drafted tokens over the paged cache on the fifth-generation tensor cores (bf16, head sizes 64 and 128).
 //
 // What a node sees, and its formula: attn_tree.cu. The query rows of a request and kv head are its nodes times the group's heads
-// (row = node x group + head), so that one pass over the keys serves the whole group: a unit of work is one (request, kv head, tile
-// of up to 128 rows, range of keys), a tile being whole nodes. Q comes with one 3-D TMA box (64 dims, the group's heads, nodes) per
-// half of the head; keys and values as in attn_prefill_tc.cu, from which the rest of the pipeline is taken too: K and V tiles of
-// 128 keys gathered page by page into a ring of three stages, S = Q K^T and O += P V as tcgen05.mma issued by one thread each, S, P
-// (bf16) and O in tensor memory, two groups of four softmax warps that take key tiles in turn and pass a row's exponent offset on,
-// an offset that moves only when the maximum has grown by more than 2^8.
-// What bounds it: up to one tile of rows per kv head the keys and values (a tile of 128 keys is 64 KB, 1.5 us at a
-// 148th of the memory's rate, against some 0.5 us for its products and softmax); with more rows the two products
-// (about 1,000 cycles for 128 x 128 x 128 each way, the softmax of one group just beside it).
+// (row = node x group + head), in tiles of up to 128 rows that are whole nodes, so that one pass over the keys serves the whole
+// group. Q comes with one 3-D TMA box (64 dims, the group's heads, nodes) per half of the head; keys and values come in tiles of
+// 64 keys, gathered page by page with 4-D boxes (128-byte swizzle) into one ring of tiles. S = Q K^T and O += P V are tcgen05.mma,
+// each kind issued by one thread; P goes to tensor memory as bf16, over the S that it was made from, and is the A operand of the
+// second product. Eight softmax warps, two threads per row with half of a tile's keys each, have two S/P buffers, so that the next
+// tile's scores are there when a tile's weights are done. A row's exponent offset moves only when its maximum has grown by more
+// than 2^8, and only then do its two threads tell each other their maxima.
+// What bounds it: a tile of keys and values is 32 KB, 0.74 us at a 148th of the memory's rate. Its 64 exponentials a row take 512
+// cycles on a unit that makes 16 a cycle, but the way from tensor memory and back and the waits between the stages take longer
+// (with four softmax warps a tile took 2,090 cycles). So two CTAs share an SM, each with half of its tensor memory and shared memory:
+// while one begins or ends a unit or waits for a product, the other one works.
 //
-// Keys are cut into as many ranges per request as fill the SMs (osb_attn_tree_tc_splits); a range leaves its unnormalised fp32
-// output, maximum and sum in scratch, laid out [4 dims][row] so that neighbouring threads (rows) write neighbouring 16 bytes straight
-// from tensor memory, and a second kernel joins them in order. The CTAs of one launch never wait for one another.
+// The work is cut evenly: all key tiles of all units (request, kv head, row tile) stand in one line, and every CTA takes an equal
+// piece of it: the end of one unit, some whole ones, the beginning of another. Every CTA finds its piece itself from the
+// requests' lengths. A unit that was cut leaves its unnormalised fp32 output, maximum and sum in scratch, two places per
+// CTA, laid out [4 dims][row] so that neighbouring threads (rows) write neighbouring 16 bytes straight from tensor memory; a second
+// kernel joins them in order. CTAs of one launch never wait for one another. A single request with several row tiles is the
+// exception in the order: its row tiles go to neighbouring CTAs that take the same keys at the same time, so that the keys of a long
+// context, more than the L2 holds, are fetched from memory once.
 //
 // Masks. A tile of keys that are all committed and inside every row's window needs none. Otherwise a row's 128 bits come from its
 // mask words (places before the tree count as ones). P is 0 where a row does not see a key, but 0 times a NaN or an infinity in V
 // would still reach the row through the tensor core: in such tiles the values that are not finite are replaced by zeros in shared
 // memory, and if there were any, the rows that do see them get them added at the end, from the cache.
+//
+// All mbarrier waits are bounded; on a time-out the CTA records a code in *err, waits for its copies in flight, frees its tensor
+// memory and returns.
 #include "attn_tree.cuh"
 #include "tc_utils.cuh"
 
@@ -26,16 +35,19 @@ namespace {
 using namespace tc;
 using namespace attn_tree;
 
-constexpr int BLOCK_M = 128, TILE_N = 128;
-constexpr int NUM_THREADS = 384;
-constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 64;   // 256 x 216 + 128 x 64 registers of the 64 K
-constexpr int STAGES = 3;  // K and V tiles in flight
-constexpr int ATOM_BYTES = 128 * 128;  // 128 rows of 128 bytes
+constexpr int BLOCK_M = 128, TILE_N = 64;
+constexpr int NUM_THREADS = 384, CTAS_PER_SM = 2;
+constexpr int Q_ATOM = BLOCK_M * 128, KV_ATOM = TILE_N * 128;   // rows of 128 bytes
+constexpr int MIN_PIECE = 2;                         // key tiles of a CTA at least
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float RESCALE_THRESHOLD = 8.0f;  // in log2 units
-constexpr int MAX_TC_SPLITS = 64;
+constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 
-// The step and how it is cut, the same for every item.
+// A unit that was cut, by the CTA in which it begins: its first token, kv head, rows and number of pieces (0: no such unit).
+struct Cut {
+  int tok0, kvh, rows, pieces;
+};
+
+// The step, the same for every CTA.
 struct Plan {
   const int* block_table;
   const int* cu_q;
@@ -43,85 +55,126 @@ struct Plan {
   const unsigned* mask;
   const int* depth;
   int* err;
+  Cut* cuts;           // scratch, by CTA
   int bt_stride, mask_words, S, nh, nkv, grp, log2ps, num_pages, window, max_q_len, kv_cap;
-  int nodes_per_tile, m_tiles, splits, chunk_tiles, n_items;
+  int nodes_per_tile, m_tiles;
+  int abreast;                      // row tiles that neighbouring CTAs take at the same time (1: row tiles are units like others)
+  unsigned inv_nodes, inv_grp;      // 2^32 / nodes_per_tile and / grp, rounded up
 };
-
-// Key tiles that a request's rows look at: the first, how many, and into how many ranges of how many tiles they are cut.
-struct Cut {
-  int first, count, ranges, per;
-};
-__device__ __forceinline__ Cut cut_of(const Plan& p, int kv_len, int base) {
-  const int lo = p.window > 0 && base - p.window + 1 > 0 ? min(base - p.window + 1, kv_len - 1) : 0;
-  Cut c;
-  c.first = lo / TILE_N;
-  c.count = (kv_len - 1) / TILE_N - c.first + 1;
-  c.ranges = min(p.splits, (c.count + p.chunk_tiles - 1) / p.chunk_tiles);
-  c.per = (c.count + c.ranges - 1) / c.ranges;
-  c.ranges = (c.count + c.per - 1) / c.per;
-  return c;
+// x / d for x below 2^25 and d up to 128, inv = ceil(2^32 / d) (d = 1: 0)
+__device__ __forceinline__ int div_by(int x, unsigned inv) { return inv == 0 ? x : (int)__umulhi((unsigned)x, inv); }
+// x / d where the quotient is below 2^20: a division in fp32, put right by one at most
+__device__ __forceinline__ int small_quotient(int x, int d) {
+  int q = (int)__fdividef((float)x, (float)d);
+  const int r = x - q * d;
+  if (r < 0) --q;
+  else if (r >= d) ++q;
+  return q;
 }
 
-// One unit of work.
-struct Item {
-  int s, kvh, node0, q0, n, rows, kv_len, base, tile_begin, n_tiles, ranges;
+// What a request brings: its key tiles and its row tiles.
+struct Req {
+  int q0, n, kv_len, base, first_tile, tiles, m_tiles;
+};
+__device__ __forceinline__ Req req_of(const Plan& p, int s) {
+  Req r;
+  r.q0 = p.cu_q[s];
+  const int q1 = p.cu_q[s + 1], kv_all = p.seq_lens[s];
+  r.n = q1 - r.q0;
+  r.kv_len = min(kv_all, p.kv_cap);
+  r.base = kv_all - r.n;
+  const int lo = p.window > 0 && r.base - p.window + 1 > 0 ? min(r.base - p.window + 1, r.kv_len - 1) : 0;
+  r.first_tile = lo / TILE_N;
+  r.tiles = r.n > 0 && r.kv_len > 0 ? (r.kv_len - 1) / TILE_N - r.first_tile + 1 : 0;
+  r.m_tiles = min(div_by(max(min(r.n, p.max_q_len), 0) + p.nodes_per_tile - 1, p.inv_nodes), p.m_tiles);
+  return r;
+}
+__device__ __forceinline__ int units_of(const Plan& p, const Req& r) { return p.abreast > 1 ? 1 : r.m_tiles; }   // per kv head
+__device__ __forceinline__ int tiles_of(const Plan& p, const Req& r) { return r.tiles > 0 ? p.nkv * units_of(p, r) * r.tiles : 0; }
+
+// One stretch of a CTA's piece: key tiles of one unit.
+struct Seg {
+  Req r;
+  int kvh, node0, rows;         // the row tile: its first node, its number of rows
+  int tile_begin, n_tiles;
+  bool whole, began;            // whole: all the unit's tiles; began: the unit began in an earlier piece
+  int pieces;                   // of a unit that begins here and is cut
   const int* bt;
 };
 
-// idx = ((request x kv heads + head) x ranges + range) x row tiles + tile: the tiles of one range run side by side, and the second to
-// read its keys finds them in the L2
-__device__ __forceinline__ bool item_of(int idx, Item& it, const Plan& p) {
-  const int m = idx % p.m_tiles;
-  idx /= p.m_tiles;
-  const int range = idx % p.splits;
-  idx /= p.splits;
-  it.kvh = idx % p.nkv;
-  it.s = idx / p.nkv;
-  it.q0 = p.cu_q[it.s];
-  it.n = p.cu_q[it.s + 1] - it.q0;
-  it.node0 = m * p.nodes_per_tile;
-  if (it.node0 >= it.n) return false;
-  const int kv_all = p.seq_lens[it.s];
-  it.kv_len = min(kv_all, p.kv_cap);
-  it.base = kv_all - it.n;
-  if (it.kv_len <= 0) {
-    atomicExch(p.err, ERR_BOUNDS);
-    return false;
+// Walks over the stretches of the piece [g, hi) of the line; `s`, `p_s`: a request and where its units begin, at or before g.
+struct Walk {
+  int g, hi, s, p_s;
+  int m, piece;                 // this CTA's row tile where row tiles go abreast; the tiles of a piece
+  Req r;                        // of request s
+  __device__ __forceinline__ bool next(const Plan& p, Seg& seg) {
+    if (g >= hi) return false;
+    for (;;) {
+      const int mine = tiles_of(p, r);
+      if (g < p_s + mine) break;
+      p_s += mine;
+      if (++s >= p.S) return false;
+      r = req_of(p, s);
+    }
+    const int unit = small_quotient(g - p_s, r.tiles), t0 = g - p_s - unit * r.tiles, units = units_of(p, r);
+    seg.r = r;
+    seg.kvh = units == 1 ? unit : small_quotient(unit, units);
+    seg.node0 = (p.abreast > 1 ? m : unit - seg.kvh * units) * p.nodes_per_tile;
+    seg.rows = min(p.nodes_per_tile, r.n - seg.node0) * p.grp;
+    seg.n_tiles = min(r.tiles - t0, hi - g);
+    seg.tile_begin = r.first_tile + t0;
+    seg.whole = seg.n_tiles == r.tiles;
+    seg.began = t0 > 0;
+    seg.pieces = 1 + (r.tiles - seg.n_tiles + piece - 1) / piece;
+    seg.bt = p.block_table + (size_t)s * p.bt_stride;
+    g += seg.n_tiles;
+    return true;
   }
-  const Cut c = cut_of(p, it.kv_len, it.base);
-  if (range >= c.ranges) return false;
-  it.ranges = c.ranges;
-  it.tile_begin = c.first + range * c.per;
-  it.n_tiles = min(c.per, c.count - range * c.per);
-  it.rows = min(p.nodes_per_tile, it.n - it.node0) * p.grp;
-  it.bt = p.block_table + (size_t)it.s * p.bt_stride;
-  return true;
-}
+};
 
 // Whether some row does not see some key of the tile from key0 on (depths are below the number of nodes).
-__device__ __forceinline__ bool tile_masked(const Item& it, const Plan& p, int key0) {
-  return key0 + TILE_N > min(it.base, it.kv_len) || (p.window > 0 && key0 < it.base + it.n - p.window);
+__device__ __forceinline__ bool tile_masked(const Req& r, const Plan& p, int key0) {
+  return key0 + TILE_N > min(r.base, r.kv_len) || (p.window > 0 && key0 < r.base + r.n - p.window);
 }
 
 // Which of the keys key0 .. key0 + 31 row `t` of the step sees; lo: the first place inside its window.
-__device__ __forceinline__ unsigned sees32(const Item& it, const Plan& p, int t, int lo, int key0) {
-  const int off = key0 - it.base;                       // of the tree's node numbers
+__device__ __forceinline__ unsigned sees32(const Req& r, const Plan& p, int t, int lo, int key0) {
+  const int off = key0 - r.base;                        // of the tree's node numbers
   const unsigned* row = p.mask + (size_t)t * p.mask_words;
   auto word = [&](int i) -> unsigned { return i < 0 ? 0xffffffffu : i < p.mask_words ? row[i] : 0u; };
   unsigned v = __funnelshift_r(word(off >> 5), word((off >> 5) + 1), off & 31);
-  const int left = it.kv_len - key0;
+  const int left = r.kv_len - key0;
   v = left >= 32 ? v : left > 0 ? v & ((1u << left) - 1u) : 0u;
   if (p.window > 0) {
-    const int hidden = min(lo, it.base) - key0;         // committed keys in front of the window
+    const int hidden = min(lo, r.base) - key0;          // committed keys in front of the window
     v = hidden >= 32 ? 0u : hidden > 0 ? v & (0xffffffffu << hidden) : v;
-    if (lo > it.base) {                                 // a window shorter than the path: ancestors by their depth
+    if (lo > r.base) {                                  // a window shorter than the path: ancestors by their depth
       for (unsigned w = v; w != 0; w &= w - 1) {
         const int j = off + __ffs(w) - 1;
-        if (j >= 0 && it.base + p.depth[it.q0 + j] < lo) v &= ~(w & (0u - w));
+        if (j >= 0 && r.base + p.depth[r.q0 + j] < lo) v &= ~(w & (0u - w));
       }
     }
   }
   return v;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  return (uint64_t)__float_as_uint(lo) | ((uint64_t)__float_as_uint(hi) << 32);
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  lo = __uint_as_float((uint32_t)v);
+  hi = __uint_as_float((uint32_t)(v >> 32));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 // Bits 15 and 31 say which of two bf16 are not finite.
@@ -131,24 +184,20 @@ __device__ __forceinline__ uint32_t without_not_finite(uint32_t w) {
   return w & ~((b & 0x8000u ? 0xffffu : 0u) | (b & 0x80000000u ? 0xffff0000u : 0u));
 }
 
-// Adds to a row's 32 outputs from column c0 on what was taken out of the V tiles: the values that are not finite of the keys that it
+// What was taken out of the V tile from key0 on for 8 dims of a row: the values that are not finite among the keys that the row
 // sees, from the cache. Only reached when a masked tile held such values.
-__device__ __noinline__ void add_not_finite(uint32_t (&o)[32], const Item& it, const Plan& p, int tok, int lo, const bf16* v_cache,
-                                            int hd, int c0) {
-  for (int t = 0; t < it.n_tiles; ++t) {
-    const int tile0 = (it.tile_begin + t) * TILE_N;
-    if (!tile_masked(it, p, tile0)) continue;
-    for (int k0 = tile0; k0 < tile0 + TILE_N; k0 += 32)
-      for (unsigned w = sees32(it, p, tok, lo, k0); w != 0; w &= w - 1) {
-        const int key = k0 + __ffs(w) - 1, page = it.bt[key >> p.log2ps];
-        if (page < 0 || page >= p.num_pages) continue;
-        const int off = key & ((1 << p.log2ps) - 1);
-        const bf16* v = v_cache + ((((size_t)page * p.nkv + it.kvh) << p.log2ps) + off) * hd + c0;
-        for (int j = 0; j < 32; ++j) {
-          const float f = __bfloat162float(v[j]);
-          if (!(fabsf(f) < INFINITY)) o[j] = __float_as_uint(__uint_as_float(o[j]) + f);
-        }
-      }
+__device__ __forceinline__ void add_taken_out(float (&x)[8], unsigned sees, int key0, const int* bt, const Plan& p, int kvh,
+                                              const bf16* v_cache, int hd, int d) {
+  for (; sees != 0; sees &= sees - 1) {
+    const int key = key0 + __ffs(sees) - 1, page = bt[key >> p.log2ps];
+    if (page < 0 || page >= p.num_pages) continue;
+    const int off = key & ((1 << p.log2ps) - 1);
+    const bf16* v = v_cache + ((((size_t)page * p.nkv + kvh) << p.log2ps) + off) * hd + d;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const float f = __bfloat162float(v[e]);
+      if (!(fabsf(f) < INFINITY)) x[e] += f;
+    }
   }
 }
 
@@ -165,426 +214,467 @@ __device__ __forceinline__ bool softmax_bar_or(bool v) {
       : "memory");
   return r != 0;
 }
+// The same for the two warps that share 32 rows.
+__device__ __forceinline__ bool pair_bar_or(int quarter, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, 64, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "r"(3 + quarter)
+      : "memory");
+  return r != 0;
+}
 
 template <int HD>
-__global__ void __launch_bounds__(NUM_THREADS, 1) attn_tree_tc_kernel(
+struct Layout {
+  static constexpr int NA = HD / 64;                  // 64-element atoms along the head dimension
+  static constexpr int Q_BYTES = NA * Q_ATOM;         // [atom][128 rows][128 B]
+  static constexpr int KV_BYTES = NA * KV_ATOM;       // a K or V tile: [atom][64 rows][128 B]
+  static constexpr int STAGES = HD == 128 ? 4 : 8;    // key and value tiles in flight: 64 KB in each of the SM's two CTAs
+  static constexpr size_t SMEM = (size_t)Q_BYTES + STAGES * KV_BYTES + 1024;
+};
+
+// Barriers (u: the CTA's key tiles, counted on across stretches; S / P buffer u % 2):
+//  full / empty: a place of the ring has its tile / the products that read it have completed. Tiles pass through the ring in the
+//    order K0, K1, V0, K2, V1, .. of a stretch, numbered on across stretches: tile i is in place i % STAGES.
+//  s_full: Q K^T of key tile u is in S. p_full: its P is there (and V may be read). pv_done: P V complete, so S / P may be overwritten,
+//    and, of a stretch's last tile, O read. q_full / epi_done: a stretch's Q has landed / its output has left O and Q's place.
+template <int HD>
+__global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, float4* __restrict__ part_o,
-    float2* __restrict__ part_ml, const bf16* __restrict__ v_cache, const __grid_constant__ Plan plan, float scale_log2,
-    int* __restrict__ err) {
-  constexpr int NA = HD / 64;                 // 64-element atoms along the head dimension
-  constexpr int Q_BYTES = NA * ATOM_BYTES;    // [atom][128 rows][128 B]
-  constexpr int KV_BYTES = NA * ATOM_BYTES;   // one K or V tile: [atom][128 keys][128 B]
-  constexpr uint32_t TMEM_COLS = 512;
-  // two S buffers of 128 columns (fp32), two P buffers of 64 columns (two bf16 per column), then O
-  constexpr uint32_t S_COL0 = 0, P_COL0 = 2 * TILE_N, O_COL = 3 * TILE_N;
+    float2* __restrict__ part_ml, const bf16* __restrict__ v_cache, const __grid_constant__ Plan plan, float scale_log2) {
+  constexpr int NA = Layout<HD>::NA, Q_BYTES = Layout<HD>::Q_BYTES, KV_BYTES = Layout<HD>::KV_BYTES, STAGES = Layout<HD>::STAGES;
+  constexpr uint32_t TMEM_COLS = 256, O_COL = 2 * TILE_N;    // S and over it P of buffer b in columns 64 b on, O in 128 on
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* q_smem = base;
-  unsigned char* k_smem = q_smem + Q_BYTES;                  // STAGES tiles
-  unsigned char* v_smem = k_smem + STAGES * KV_BYTES;     // STAGES tiles
-  // The tiles a CTA works through are counted across its items: tile u uses K/V stage u % STAGES and S/P buffer u % 2.
-  // k_free / s_full: Q K^T of a tile complete (the K tile may be overwritten / S may be read);
-  // s_free: the softmax warps hold the tile's S in registers (the S buffer may be overwritten);
-  // p_full: P of a tile is in tensor memory; v_free / p_free: P V of a tile complete (the V tile / the P buffer
-  // may be overwritten, O may be read); epi_done: an item's output has left tensor and shared memory (the next
-  // item's Q may be loaded; its first P V, which overwrites O, follows from that)
-  __shared__ uint64_t q_full, epi_done, k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES];
-  __shared__ uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
-  // max_done[u % 2]: the rows' exponent offsets after tile u are in row_offset (the group of tile u + 1 may go on)
-  __shared__ uint64_t max_done[2];
-  __shared__ float row_offset[BLOCK_M];   // per query row: the exponent offset in use (log2 units), -inf before the first key
-  __shared__ float row_sum[2][BLOCK_M];   // per group and row: its sum of P at the final offset
+  unsigned char* ring = base + Q_BYTES;               // STAGES tiles of keys or values
+  __shared__ uint64_t q_full, epi_done, full[STAGES], empty[STAGES], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int found_bad[2];            // by the parity of the CTA's items: values that are not finite were taken out of a V tile
+  __shared__ int found_bad[2];            // by the parity of the CTA's stretches: values that are not finite were taken out of a V tile
+  __shared__ int scan[NUM_THREADS / 32];
+  __shared__ int start_s, start_p;        // the request in which this CTA's piece begins, where its units begin
+  __shared__ Req start_r;
+  __shared__ float row_max[2][2][BLOCK_M];   // by the parity of the key tile, half of the keys, row
+  __shared__ float row_sum[2][BLOCK_M];      // by half, row
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ps = 1 << plan.log2ps, log2ps = plan.log2ps;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int log2ps = plan.log2ps, ps = 1 << log2ps;
   const int box_rows = ps < TILE_N ? ps : TILE_N;  // keys per TMA box: a page, or a tile's worth of a larger page
   const int n_boxes = TILE_N / box_rows;
+  int* err = plan.err;
 
   if (lane == 0 && warp < 3) prefetch_tensormap(warp == 0 ? &map_k : warp == 1 ? &map_q : &map_v);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     abort_flag = 0;
     found_bad[0] = found_bad[1] = 0;
+    start_s = 0;
     mbar_init(&q_full, 1);
     mbar_init(&epi_done, 8);
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&k_free[i], 1);
-      mbar_init(&v_free[i], 1);
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&p_free[i], 1);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&pv_done[i], 1);
     }
-    mbar_init(&max_done[0], BLOCK_M);
-    mbar_init(&max_done[1], BLOCK_M);
     mbar_init_fence();
   }
-  if (threadIdx.x < BLOCK_M) row_offset[threadIdx.x] = -INFINITY;
   if (warp == 1) tmem_alloc(&tmem_slot, TMEM_COLS);
-  // until here nothing was read that the kernel before this one in the stream may still be writing (q, the pages)
+  // until here nothing was read that the kernel before this one in the stream may still be writing (lengths, q, the pages)
   pdl_wait();
+
+  // ---- this CTA's piece of the line of tiles
+  Req mine = {};                                // of request `tid`
+  int my_tiles = 0;
+  long long all = 0;
+  for (int s = tid; s < plan.S; s += NUM_THREADS) {
+    const Req r = req_of(plan, s);
+    const int t = tiles_of(plan, r);
+    if (s == tid) {
+      mine = r;
+      my_tiles = t;
+    }
+    all += t;
+    if (blockIdx.x == 0 && r.n > 0 && (r.kv_len < r.base + r.n || r.n > plan.max_q_len || r.base < 0)) atomicExch(err, ERR_BOUNDS);
+  }
+  auto block_scan = [&](int v, int& total) -> int {      // exclusive
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NUM_THREADS / 32; ++w) {
+      before += w < warp ? scan[w] : 0;
+      total += scan[w];
+    }
+    return before + inc - v;
+  };
+  int total;
+  const int first = block_scan((int)all, total);
+  // (row tiles abreast: a group of CTAs has one piece)
+  const int groups = plan.abreast > 1 ? (int)gridDim.x / plan.abreast : (int)gridDim.x;
+  const int group = plan.abreast > 1 ? (int)blockIdx.x / plan.abreast : (int)blockIdx.x;
+  const int piece = max(MIN_PIECE, (total + groups - 1) / groups);
+  const int g0 = (int)min((long long)total, (long long)group * piece), g1 = group < groups ? min(total, g0 + piece) : g0;
+  if (plan.S <= NUM_THREADS) {
+    if (my_tiles > 0 && g0 >= first && g0 < first + my_tiles) {
+      start_s = tid;
+      start_p = first;
+      start_r = mine;
+    }
+  } else {
+    int run = 0;
+    for (int s0 = 0; s0 < plan.S; s0 += NUM_THREADS) {
+      const int s = s0 + tid;
+      const int t = s < plan.S ? tiles_of(plan, req_of(plan, s)) : 0;
+      int chunk;
+      __syncthreads();                          // everyone has read the scan's words
+      const int at = run + block_scan(t, chunk);
+      if (t > 0 && g0 >= at && g0 < at + t) {
+        start_s = s;
+        start_p = at;
+        start_r = req_of(plan, s);
+      }
+      run += chunk;
+    }
+  }
+  if (tid == 128) plan.cuts[blockIdx.x].pieces = 0;      // (the thread that may say otherwise later)
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
   volatile int* vabort = &abort_flag;
-  Item it;
-  int idx = 0;
-  auto next_item = [&](int& pass) -> bool {   // the same sequence of items in every warp
-    for (;;) {
-      idx = (int)blockIdx.x + (int)gridDim.x * pass++;
-      if (idx >= plan.n_items) return false;
-      if (item_of(idx, it, plan)) return true;
-    }
-  };
+  Walk walk;
+  walk.g = g0;
+  walk.hi = g1;
+  walk.s = start_s;
+  walk.p_s = start_p;
+  walk.r = start_r;
+  walk.piece = piece;
+  walk.m = plan.abreast > 1 ? (int)blockIdx.x - group * plan.abreast : 0;
+  if (plan.abreast > 1 && walk.m >= start_r.m_tiles) walk.hi = walk.g;     // the request has fewer row tiles than it might
+  Seg seg;
 
-  if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------------ TMA producers: warp 0 keys, warp 2 values
-    const int which = warp == 0 ? 0 : 1;
-    unsigned char* tiles = which ? v_smem : k_smem;
-    const CUtensorMap* map = which ? &map_v : &map_k;
-    // lane = (box b, atom a) of a tile: boxes * NA <= 32, a box being at least 8 keys
-    const int b = lane / NA, a = lane - b * NA;
-    int u0 = 0;   // tiles of the items before this one
-    int issued = 0;
-    for (int pass = 0; next_item(pass) && !*vabort; u0 += it.n_tiles) {
-      const int p_last = it.kv_len - 1;
-      if (which == 0 && lane == 0 && (it.kv_len < it.base + it.n || it.n > plan.max_q_len || it.base < 0)) atomicExch(err, ERR_BOUNDS);
+    // Lane b looks up the page of box b; one thread issues all copies of a tile one after the other (a copy per lane would be
+    // a loop over the lanes, some 190 cycles each).
+    const bool keys = warp == 0;
+    const CUtensorMap* map = keys ? &map_k : &map_v;
+    int i0 = 0;             // tiles that were put into the ring before this stretch, by both
+    int last[2] = {-1, -1}; // numbers of the tiles that this warp put into the ring last
+    for (; !*vabort && walk.next(plan, seg); i0 += 2 * seg.n_tiles) {
+      const int p_last = seg.r.kv_len - 1;
       // a page outside the pool reads as zeros; it is reported unless every row's window has passed it (then it was given back)
       auto page_of = [&](int t) -> int {
-        const int key = (it.tile_begin + t) * TILE_N + b * box_rows;
-        if (t >= it.n_tiles || b >= n_boxes || key > p_last) return -1;
-        const int page = it.bt[key >> log2ps];
+        const int key = (seg.tile_begin + t) * TILE_N + lane * box_rows;
+        if (t >= seg.n_tiles || lane >= n_boxes || key > p_last) return -1;
+        const int page = seg.bt[key >> log2ps];
         if (page >= 0 && page < plan.num_pages) return page;
-        if (plan.window <= 0 || key + box_rows > it.base - plan.window + 1) atomicExch(err, ERR_PAGE);
+        if (plan.window <= 0 || key + box_rows > seg.r.base - plan.window + 1) atomicExch(err, ERR_PAGE);
         return -1;
       };
-      int page = page_of(0);
-      for (int t = 0; t < it.n_tiles; ++t) {
-        const int u = u0 + t, st = u % STAGES;
-        const uint32_t ph = (uint32_t)(u / STAGES) & 1u;
-        const int key0 = (it.tile_begin + t) * TILE_N;
-        const int next_page = page_of(t + 1);  // in flight while this tile's copies are issued
-        // whole boxes (pages) up to the last key this item may look at; a box that starts beyond it is skipped
+      int page = page_of(0), next_page = page_of(1);
+      for (int t = 0; t < seg.n_tiles && !*vabort; ++t) {
+        const int after_next = page_of(t + 2);  // in flight while these tiles' copies are issued
+        const int i = i0 + (keys ? (t == 0 ? 0 : 2 * t - 1) : (t + 1 < seg.n_tiles ? 2 * t + 2 : 2 * t + 1)), st = i % STAGES;
+        const int key0 = (seg.tile_begin + t) * TILE_N;
+        // whole boxes (pages) up to the request's last key; a box that starts beyond it is skipped
         const int boxes = min(n_boxes, (p_last - key0) / box_rows + 1);
-        uint64_t* empty = which ? &v_free[st] : &k_free[st];
-        uint64_t* full = which ? &v_full[st] : &k_full[st];
         if (lane == 0) {
-          if (!mbar_wait(empty, ph ^ 1u, vabort)) {
+          if (!mbar_wait(&empty[st], ((uint32_t)(i / STAGES) & 1u) ^ 1u, vabort)) {
             if (!*vabort) atomicExch(err, 111);
             *vabort = 1;
           } else {
-            mbar_expect_tx(full, (uint32_t)(boxes * NA * box_rows * 128));
+            mbar_expect_tx(&full[st], (uint32_t)(boxes * NA * box_rows * 128));
           }
         }
         __syncwarp();
         if (*vabort) break;
-        if (lane < boxes * NA)
-          tma_load_4d(tiles + st * KV_BYTES + a * ATOM_BYTES + b * box_rows * 128, map, full, a * 64,
-                      (key0 + b * box_rows) & (ps - 1), it.kvh, page);
+        unsigned char* to = ring + st * KV_BYTES;
+        const int row0 = key0 & (ps - 1);       // of the first box in its page (the others begin a page)
+#pragma unroll 2
+        for (int b = 0; b < boxes; ++b) {
+          const int pg = __shfl_sync(0xffffffffu, page, b);
+          if (lane == 0) {
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+              tma_load_4d(to + a * KV_ATOM + b * box_rows * 128, map, &full[st], a * 64, (row0 + b * box_rows) & (ps - 1), seg.kvh, pg);
+          }
+        }
+        last[0] = last[1];
+        last[1] = i;
         page = next_page;
-        issued = u + 1;
+        next_page = after_next;
       }
     }
-    // after a failure: every copy that was issued lands before the CTA goes (a tile's barrier completes with it)
+    // after a failure: every copy that was issued lands before the CTA goes (a tile's barrier completes with it; earlier
+    // ones have, since the ring came round)
     if (*vabort && lane == 0) {
-      for (int u = max(0, issued - STAGES); u < issued; ++u) {
-        uint64_t* full = which ? &v_full[u % STAGES] : &k_full[u % STAGES];
-        for (uint32_t w = 0; w < WAIT_LIMIT && !mbar_try_wait(full, (uint32_t)(u / STAGES) & 1u); ++w) {
+      for (int k = 0; k < 2; ++k)
+        for (uint32_t w = 0; last[k] >= 0 && w < WAIT_LIMIT && !mbar_try_wait(&full[last[k] % STAGES], (uint32_t)(last[k] / STAGES) & 1u); ++w) {
         }
-      }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ issuer of S = Q K^T, up to two tiles ahead
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc(BLOCK_M, TILE_N, 0, 0);
-      bool ok = true;
-      int u0 = 0, n_done = 0;
-      for (int pass = 0; ok && next_item(pass); u0 += it.n_tiles, ++n_done) {
-        ok = mbar_wait(&q_full, (uint32_t)n_done & 1u, vabort);
-        for (int t = 0; t < it.n_tiles && ok; ++t) {
-          const int u = u0 + t, st = u % STAGES;
-          // the keys have landed, and the softmax warps have taken tile u - 2 out of this S buffer
-          if (!mbar_wait(&k_full[st], (uint32_t)(u / STAGES) & 1u, vabort) ||
-              !mbar_wait(&s_free[u & 1], ((uint32_t)(u >> 1) & 1u) ^ 1u, vabort)) {
-            ok = false;
-            break;
-          }
-          fence_after();
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint64_t ad = desc_kmajor(q_smem + (ks >> 2) * ATOM_BYTES) + (uint64_t)((ks & 3) * 2);
-            const uint64_t bd = desc_kmajor(k_smem + st * KV_BYTES + (ks >> 2) * ATOM_BYTES) + (uint64_t)((ks & 3) * 2);
-            umma_bf16(tmem + S_COL0 + (uint32_t)((u & 1) * TILE_N), ad, bd, idesc_s, ks > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[u & 1]);
-          umma_commit(&k_free[st]);
-        }
-      }
-      if (!ok) {
-        if (!*vabort) atomicExch(err, 112);
-        *vabort = 1;
-      }
-    }
-  } else {
-    // ------------------------------------------------------------------ warp 3: loads Q, issues O += P V
-    if (lane == 0) {
-      constexpr uint32_t idesc_o = make_idesc(BLOCK_M, HD, 0, 1);  // B = V: N (head dim) contiguous
-      bool ok = true;
-      int u0 = 0, n_done = 0, q_issued = 0;
-      for (int pass = 0; ok && next_item(pass); u0 += it.n_tiles, ++n_done) {
-        // Q goes where the item before staged its output: wait until that has left
-        if (n_done > 0 && !mbar_wait(&epi_done, (uint32_t)(n_done - 1) & 1u, vabort)) {
-          ok = false;
-          break;
-        }
-        mbar_expect_tx(&q_full, (uint32_t)(NA * plan.nodes_per_tile * plan.grp * 128));
-        for (int a = 0; a < NA; ++a)
-          tma_load_3d(q_smem + a * ATOM_BYTES, &map_q, &q_full, a * 64, it.kvh * plan.grp, it.q0 + it.node0);
-        q_issued = n_done + 1;
-        for (int t = 0; t < it.n_tiles && ok; ++t) {
-          const int u = u0 + t, st = u % STAGES;
-          if (!mbar_wait(&p_full[u & 1], (uint32_t)(u >> 1) & 1u, vabort) ||
-              !mbar_wait(&v_full[st], (uint32_t)(u / STAGES) & 1u, vabort)) {
-            ok = false;
-            break;
-          }
-          fence_after();
-          const uint32_t p_tmem = tmem + P_COL0 + (uint32_t)((u & 1) * (TILE_N / 2));
-#pragma unroll
-          for (int ks = 0; ks < TILE_N / 16; ++ks) {
-            const uint64_t bd = desc_mnmajor(v_smem + st * KV_BYTES, ATOM_BYTES) + (uint64_t)(ks * (16 * 128 / 16));
-            umma_bf16_ts(tmem + O_COL, p_tmem + (uint32_t)(ks * 8), bd, idesc_o, (t > 0 || ks > 0) ? 1u : 0u);
-          }
-          umma_commit(&p_free[u & 1]);
-          umma_commit(&v_free[st]);
-        }
-      }
-      if (!ok) {
-        if (!*vabort) atomicExch(err, 112);
-        *vabort = 1;
-        for (uint32_t w = 0; q_issued > 0 && w < WAIT_LIMIT && !mbar_try_wait(&q_full, (uint32_t)(q_issued - 1) & 1u); ++w) {
-        }
-      }
-    }
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-    // ------------------------------------------------------------------ softmax and epilogue: two groups of four warps
-    const int grp = (warp - 4) >> 2;     // group 0 takes the even tiles of the CTA's count, group 1 the odd ones
-    const int qd = warp & 3;             // TMEM lane quarter of this warp
-    const int r = qd * 32 + lane;        // query row of this thread
-    const uint32_t lane_addr = (uint32_t)(qd * 32) << 16;
-    const uint32_t s_addr = tmem + lane_addr + S_COL0 + (uint32_t)(grp * TILE_N);
-    const uint32_t p_addr = tmem + lane_addr + P_COL0 + (uint32_t)(grp * (TILE_N / 2));
-    int u0 = 0, n_done = 0;
-    bool stop = false;
-    for (int pass = 0; !stop && next_item(pass); u0 += it.n_tiles, ++n_done) {
-      const int tok = r < it.rows ? it.q0 + it.node0 + r / plan.grp : -1;   // this row's token, or none
-      int lo_row = 0;
-      if (plan.window > 0 && tok >= 0) lo_row = it.base + min(max(plan.depth[tok], 0), it.n - 1) - plan.window + 1;
-      const int u_last = u0 + it.n_tiles - 1;
-      // my_off: the offset this thread's sum l_run is expressed at (what it last saw or set)
-      float my_off = -INFINITY, l_run = 0.0f;
-      bool ok = true;
-      for (int t = (u0 & 1) == grp ? 0 : 1; t < it.n_tiles; t += 2) {
-        const int u = u0 + t;                             // u % 2 == grp
-        const uint32_t ph2 = (uint32_t)(u >> 1) & 1u;     // phase of this group's S/P barriers
-        const int key0 = (it.tile_begin + t) * TILE_N;
-        const bool masked = tile_masked(it, plan, key0);
-        unsigned sees[4] = {0u, 0u, 0u, 0u};
-        if (masked && tok >= 0) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sees[c] = sees32(it, plan, tok, lo_row, key0 + c * 32);
-        }
-        if (!mbar_wait(&s_full[grp], ph2, vabort)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+    // ------------------------------------------------------------------ issuer of S = Q K^T
+    // (the whole warp goes through the loops, one thread issues: the descriptors then stay in uniform registers)
+    constexpr uint32_t idesc_s = make_idesc(BLOCK_M, TILE_N, 0, 0);
+    const uint64_t q_desc = desc_kmajor(q_smem), k_desc = desc_kmajor(ring);
+    bool ok = true;
+    int i0 = 0, n_done = 0, u = 0;
+    for (; ok && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
+      ok = mbar_wait(&q_full, (uint32_t)n_done & 1u, vabort);
+      for (int t = 0; t < seg.n_tiles; ++t, ++u) {
+        const int i = i0 + (t == 0 ? 0 : 2 * t - 1), st = i % STAGES, b = u & 1;
+        // the keys have landed, and P V of the tile before the last has completed: its S / P may be overwritten
+        ok = ok && mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1u, vabort) &&
+             (u < 2 || mbar_wait(&pv_done[b], (uint32_t)((u >> 1) - 1) & 1u, vabort));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         fence_after();
-        uint32_t v[4][32];
+        const uint64_t bd = k_desc + (uint64_t)((st * KV_BYTES) >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + (uint32_t)(c * 32), v[c]);
-        tmem_ld_wait();
-        // the row is in registers: the S buffer is free for the tile after the next
-        fence_before();
+          for (int ks = 0; ks < HD / 16; ++ks)
+            umma_bf16(tmem + (uint32_t)(b * TILE_N), q_desc + (uint64_t)((ks >> 2) * (Q_ATOM >> 4) + (ks & 3) * 2),
+                      bd + (uint64_t)((ks >> 2) * (KV_ATOM >> 4) + (ks & 3) * 2), idesc_s, ks > 0 ? 1u : 0u);
+          umma_commit(&s_full[b]);
+          umma_commit(&empty[st]);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[grp]);
+      }
+    }
+    if (!ok && lane == 0) {
+      if (!*vabort) atomicExch(err, 112);
+      *vabort = 1;
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ loads Q, issues O += P V
+    constexpr uint32_t idesc_o = make_idesc(BLOCK_M, HD, 0, 1);  // B = V: N (head dim) contiguous
+    const uint64_t v_desc = desc_mnmajor(ring, KV_ATOM);
+    bool ok = true;
+    int i0 = 0, n_done = 0, q_issued = 0, u = 0;
+    for (; ok && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
+      // Q goes where the stretch before staged its output: wait until that has left
+      if (n_done > 0 && !mbar_wait(&epi_done, (uint32_t)(n_done - 1) & 1u, vabort)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(&q_full, (uint32_t)(NA * plan.nodes_per_tile * plan.grp * 128));
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+          tma_load_3d(q_smem + a * Q_ATOM, &map_q, &q_full, a * 64, seg.kvh * plan.grp, seg.r.q0 + seg.node0);
+      }
+      __syncwarp();
+      q_issued = n_done + 1;
+      for (int t = 0; t < seg.n_tiles; ++t, ++u) {
+        const int i = i0 + (t + 1 < seg.n_tiles ? 2 * t + 2 : 2 * t + 1), st = i % STAGES, b = u & 1;
+        ok = mbar_wait(&p_full[b], (uint32_t)(u >> 1) & 1u, vabort) && mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1u, vabort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        const uint64_t bd = v_desc + (uint64_t)((st * KV_BYTES) >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < TILE_N / 16; ++ks)
+            umma_bf16_ts(tmem + O_COL, tmem + (uint32_t)(b * TILE_N + ks * 8), bd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o,
+                         (t > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&pv_done[b]);
+          umma_commit(&empty[st]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      if (lane == 0) {
+        if (!*vabort) atomicExch(err, 112);
+        *vabort = 1;
+      }
+      for (uint32_t w = 0; q_issued > 0 && w < WAIT_LIMIT && !mbar_try_wait(&q_full, (uint32_t)(q_issued - 1) & 1u); ++w) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax and epilogue: eight warps
+    const int qd = warp & 3;             // TMEM lane quarter of this warp
+    const int half = (warp - 4) >> 2;    // of a tile's keys, and of the output's columns
+    const int r = qd * 32 + lane;        // query row of this thread
+    const int ts = tid - 128;
+    const uint32_t s_addr = tmem + ((uint32_t)(qd * 32) << 16), o_addr = s_addr + O_COL + (uint32_t)(half * (HD / 2));
+    int i0 = 0, n_done = 0, u = 0;
+    bool stop = false;
+    for (; !stop && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
+      const int tok = r < seg.rows ? seg.r.q0 + seg.node0 + div_by(r, plan.inv_grp) : -1;   // this row's token, or none
+      int lo_row = 0;
+      if (plan.window > 0 && tok >= 0) lo_row = seg.r.base + min(max(plan.depth[tok], 0), seg.r.n - 1) - plan.window + 1;
+      float m_run = -INFINITY, l_run = 0.0f;       // the row's exponent offset in use and the sum at it over this half's keys
+      bool ok = true;
+      for (int t = 0; t < seg.n_tiles; ++t, ++u) {
+        const int key0 = (seg.tile_begin + t) * TILE_N, b = u & 1;
+        const bool masked = tile_masked(seg.r, plan, key0);
+        unsigned sees = 0u;
+        if (masked && tok >= 0) sees = sees32(seg.r, plan, tok, lo_row, key0 + half * 32);
+        if (!mbar_wait(&s_full[b], (uint32_t)(u >> 1) & 1u, vabort)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        const uint32_t sb = s_addr + (uint32_t)(b * TILE_N);
+        uint32_t v[32];
+        tmem_ld32(sb + (uint32_t)(half * 32), v);
+        tmem_ld_wait();
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int j = 0; j < 32; ++j)
+            if (!((sees >> j) & 1u)) v[j] = 0xff800000u;  // -inf
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!((sees[c] >> j) & 1u)) v[c][j] = 0xff800000u;  // -inf
-        }
-        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+        for (int j = 0; j < 32; j += 8)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          mx0 = fmaxf(mx0, __uint_as_float(v[0][j]));
-          mx1 = fmaxf(mx1, __uint_as_float(v[1][j]));
-          mx2 = fmaxf(mx2, __uint_as_float(v[2][j]));
-          mx3 = fmaxf(mx3, __uint_as_float(v[3][j]));
-        }
-        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * scale_log2;  // the scale is positive
-        // the row's offset after the tile before, which the other group's thread of this row has set
-        if (t > 0) {
-          if (!mbar_wait(&max_done[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u, vabort)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-        }
-        const float m_used = row_offset[r];   // -inf at an item's first tile
-        // the exponent offset in use moves only when the maximum has grown enough (or at the first keys)
-        const bool grow = mx > m_used + RESCALE_THRESHOLD || (m_used == -INFINITY && mx > -INFINITY);
-        const float m_new = grow ? mx : m_used;
-        row_offset[r] = m_new;
-        mbar_arrive(&max_done[grp]);    // releases the write above to the thread that waits for this tile's offsets
-        // this thread's sum at the new offset: first to what the other group left, then to what this tile sets
-        if (my_off != m_new) l_run = my_off == -INFINITY ? 0.0f : l_run * ex2_approx(my_off - m_new);
-        my_off = m_new;
-        const float alpha = (grow && m_used != -INFINITY) ? ex2_approx(m_used - m_new) : 1.0f;
-        if (t > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-          // O belongs to the tensor cores until the product of the tile before has completed; the product of this
-          // tile waits for this thread's P, the products after it for this one: nothing else touches O meanwhile
-          if (!mbar_wait(&p_free[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u, vabort)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          fence_after();
+          for (int e = 0; e < 4; ++e)
+            mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;  // the scale is positive
+        // the exponent offset in use moves only when the maximum has grown enough (or at the first keys); what lies in rows
+        // that are none moves nothing. (The barrier also says that both warps have read their scores: P goes over them.)
+        bool grow = tok >= 0 && (mx > m_run + RESCALE_THRESHOLD || (m_run == -INFINITY && mx > -INFINITY));
+        if (pair_bar_or(qd, grow)) {
+          row_max[b][half][r] = mx;
+          pair_bar_or(qd, false);
+          mx = fmaxf(mx, row_max[b][half ^ 1][r]);
+          grow = tok >= 0 && (mx > m_run + RESCALE_THRESHOLD || (m_run == -INFINITY && mx > -INFINITY));
+          const float alpha = (grow && m_run != -INFINITY) ? ex2_approx(m_run - mx) : 1.0f;
+          if (grow) m_run = mx;
+          if (t > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            // once the tile before has left the tensor cores nothing else touches O until all P of this one is there
+            if (!mbar_wait(&pv_done[b ^ 1], (uint32_t)((u - 1) >> 1) & 1u, vabort)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+              fence_after();
+              l_run *= alpha;
 #pragma unroll 1
-          for (int c0 = 0; c0 < HD; c0 += 32) {
-            uint32_t o[32];
-            tmem_ld32(tmem + lane_addr + O_COL + (uint32_t)c0, o);
-            tmem_ld_wait();
+              for (int c0 = 0; c0 < HD / 2; c0 += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + (uint32_t)c0, o);
+                tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_st32(tmem + lane_addr + O_COL + (uint32_t)c0, o);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                tmem_st16(o_addr + (uint32_t)c0, o);
+              }
+            }
           }
         }
-        // the product that read this P buffer last (tile u - 2) has completed
-        if (u >= 2) {
-          if (!mbar_wait(&p_free[grp], ph2 ^ 1u, vabort)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          fence_after();
-        }
-        // P = exp2(S * scale - offset), two bf16 per column of this group's P buffer;
+        // P = exp2(S * scale - offset), two bf16 per column, over the S that was read;
         // rows that have seen no key yet (offset -inf) are all masked here: exp2(-inf) = 0 with any finite offset
-        const float offset = m_new == -INFINITY ? 0.0f : m_new;
-        float sum0 = 0.0f, sum1 = 0.0f;
+        const float offset = m_run == -INFINITY ? 0.0f : m_run;
+        const uint64_t scale2 = pack2(scale_log2, scale_log2), offset2 = pack2(-offset, -offset);
+        uint64_t sum_a = 0ull, sum_b = 0ull;
+        uint32_t pk[16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(v[c][j]), scale_log2, -offset));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(v[c][j + 1]), scale_log2, -offset));
-            sum0 += p0;
-            sum1 += p1;
-            __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
-            v[c >> 1][(c & 1) * 16 + (j >> 1)] = *reinterpret_cast<uint32_t*>(&b);
-          }
-          if (c == 1) tmem_st32(p_addr, v[0]);
+        for (int j = 0; j < 32; j += 2) {
+          float x, y;
+          unpack2(fma2((uint64_t)v[j] | ((uint64_t)v[j + 1] << 32), scale2, offset2), x, y);
+          const float p0 = ex2_approx(x), p1 = ex2_approx(y);
+          if (j & 2) sum_b = add2(sum_b, pack2(p0, p1));
+          else sum_a = add2(sum_a, pack2(p0, p1));
+          __nv_bfloat162 w = __floats2bfloat162_rn(p0, p1);
+          pk[j >> 1] = *reinterpret_cast<uint32_t*>(&w);
         }
-        tmem_st32(p_addr + 32u, v[1]);
-        l_run += sum0 + sum1;
+        tmem_st16(sb + (uint32_t)(half * 16), pk);
+        float s0, s1;
+        unpack2(add2(sum_a, sum_b), s0, s1);
+        l_run += s0 + s1;
         // V of a masked tile: rows from the first key that was not loaded (shared memory never written, or an older tile) or that
         // lies at or beyond the request's length (whatever the page held before) are cleared, and so is every value that is
-        // not finite: P = 0 must hide it
+        // not finite: P = 0 must hide it. A thread has a quarter of one key's row.
         if (masked) {
-          const int loaded = min(n_boxes, (it.kv_len - 1 - key0) / box_rows + 1) * box_rows;
-          const int first_bad = min(it.kv_len - key0, loaded);
-          const int st = u % STAGES;
-          if (!mbar_wait(&v_full[st], (uint32_t)(u / STAGES) & 1u, vabort)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          unsigned char* vrow = v_smem + st * KV_BYTES + r * 128;
-          if (r >= first_bad) {
-            for (int a = 0; a < NA; ++a)
+          const int i = i0 + (t + 1 < seg.n_tiles ? 2 * t + 2 : 2 * t + 1), st = i % STAGES;
+          const int loaded = min(n_boxes, (seg.r.kv_len - 1 - key0) / box_rows + 1) * box_rows;
+          const int first_bad = min(seg.r.kv_len - key0, loaded);
+          if (ok && !mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1u, vabort)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            const int row = ts & (TILE_N - 1), c0 = (ts / TILE_N) * (2 * NA);     // 16-byte pieces c0 .. c0 + 2 NA - 1 of 8 NA
+            unsigned char* vrow = ring + st * KV_BYTES + row * 128;
+            auto piece_at = [&](int c) { return reinterpret_cast<uint4*>(vrow + (c >> 3) * KV_ATOM + (((c ^ row) & 7) << 4)); };
+            if (row >= first_bad) {
 #pragma unroll
-              for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vrow + a * ATOM_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
-          } else {
-            uint32_t any = 0u;
+              for (int c = 0; c < 2 * NA; ++c) *piece_at(c0 + c) = make_uint4(0, 0, 0, 0);
+            } else {
+              uint32_t any = 0u;
 #pragma unroll
-            for (int c = 0; c < 8 * NA; ++c) {
-              const uint4 w = *reinterpret_cast<const uint4*>(vrow + (c >> 3) * ATOM_BYTES + (((c ^ r) & 7) << 4));
-              any |= not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
-            }
-            if (any) {
-              for (int c = 0; c < 8 * NA; ++c) {
-                uint4* at = reinterpret_cast<uint4*>(vrow + (c >> 3) * ATOM_BYTES + ((c & 7) << 4));
-                uint4 w = *at;
-                w.x = without_not_finite(w.x);
-                w.y = without_not_finite(w.y);
-                w.z = without_not_finite(w.z);
-                w.w = without_not_finite(w.w);
-                *at = w;
+              for (int c = 0; c < 2 * NA; ++c) {
+                const uint4 w = *piece_at(c0 + c);
+                any |= not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
               }
-              found_bad[n_done & 1] = 1;
+              if (any) {
+                found_bad[n_done & 1] = 1;
+#pragma unroll 1
+                for (int c = 0; c < 2 * NA; ++c) {
+                  uint4 w = *piece_at(c0 + c);
+                  w.x = without_not_finite(w.x);
+                  w.y = without_not_finite(w.y);
+                  w.z = without_not_finite(w.z);
+                  w.w = without_not_finite(w.w);
+                  *piece_at(c0 + c) = w;
+                }
+              }
             }
+            fence_async_smem();
           }
-          fence_async_smem();
         }
+        if (!ok) break;
         tmem_st_wait();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[grp]);
+        if (lane == 0) mbar_arrive(&p_full[b]);
       }
-      // both groups bring their sums to the offset after the last tile and exchange them
-      if (ok && (u_last & 1) != grp) {   // the other group had the last tile
-        if (!mbar_wait(&max_done[u_last & 1], (uint32_t)(u_last >> 1) & 1u, vabort)) ok = false;
+      // ---- epilogue, when the last product has completed
+      row_sum[half][r] = l_run;
+      if (ok && !mbar_wait(&pv_done[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u, vabort)) ok = false;
+      if (walk.g >= walk.hi) pdl_trigger();        // the last stretch of this CTA
+      stop = softmax_bar_or(!ok || *vabort != 0);
+      if (stop) {
+        if (lane == 0) {
+          if (!*vabort) atomicExch(err, 113);
+          *vabort = 1;
+        }
+        break;
       }
-      const float m_final = row_offset[r];
-      {
-        const float m_fin = m_final;
-        if (my_off != m_fin) l_run = my_off == -INFINITY ? 0.0f : l_run * ex2_approx(my_off - m_fin);
-        row_sum[grp][r] = l_run;
-      }
-      asm volatile("bar.sync 2, 256;" ::: "memory");   // the eight softmax warps
-      if (grp == 0) row_offset[r] = -INFINITY;          // for the next item; its first tile is read after the barrier below
-      if (threadIdx.x == 128) found_bad[(n_done + 1) & 1] = 0;   // last read before the barrier that ended the item before
-      if ((int)blockIdx.x + (int)gridDim.x * pass >= plan.n_items) pdl_trigger();   // the last item of this CTA
-      // epilogue. One range: O / l as bf16 through the shared memory that held Q (every product that read it has completed),
-      // each group half of the head's columns, so that the rows go out in whole 16-byte pieces side by side. Several: O as
-      // fp32 into this item's scratch.
-      constexpr int CPR = HD / 8;          // 16-byte pieces per row; piece c of row r lies at slot c ^ (r % CPR)
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && !mbar_wait(&p_free[u_last & 1], (uint32_t)(u_last >> 1) & 1u, vabort)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        fence_after();
-        const float l = row_sum[0][r] + row_sum[1][r];
-        const float inv = it.ranges > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-        const bool bad = found_bad[n_done & 1] != 0;
+      const bool cut = !seg.whole, bad = found_bad[n_done & 1] != 0;
+      const int slot = 2 * (int)blockIdx.x + (seg.began ? 0 : 1);
+      float4* po = part_o + (size_t)slot * (HD / 4) * BLOCK_M + r;
+      // One range of keys: O / l as bf16 through the shared memory that held Q (every product that read it has completed), so that
+      // the rows go out in whole lines: 16-byte piece c of row r lies at slot c ^ (r % CPR) of its row. Cut: O as fp32 to scratch.
+      constexpr int CPR = HD / 8;
+      const float l_all = row_sum[0][r] + row_sum[1][r];
+      const float inv = cut ? 1.0f : l_all == 0.0f ? 0.0f : 1.0f / l_all;
+      fence_after();
 #pragma unroll
-        for (int c0 = grp * (HD / 2); c0 < (grp + 1) * (HD / 2); c0 += 32) {
-          uint32_t o[32];
-          tmem_ld32(tmem + lane_addr + O_COL + (uint32_t)c0, o);
-          tmem_ld_wait();
-          if (bad && tok >= 0) add_not_finite(o, it, plan, tok, lo_row, v_cache, HD, c0);
-          if (it.ranges > 1) {
-            float4* po = part_o + ((size_t)idx * (HD / 4) + c0 / 4) * BLOCK_M + r;
+      for (int c0 = 0; c0 < HD / 2; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32(o_addr + (uint32_t)c0, o);
+        tmem_ld_wait();
+        const int col = half * (HD / 2) + c0;
+        if (cut) {
+          if (tok >= 0)
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
-              po[(j / 4) * BLOCK_M] = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]),
-                                                  __uint_as_float(o[j + 3]));
-            continue;
-          }
+              po[((col + j) / 4) * BLOCK_M] = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]),
+                                                          __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+        } else {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 w;
@@ -592,32 +682,54 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) attn_tree_tc_kernel(
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               hh[e] = __floats2bfloat162_rn(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
-            const int c = (c0 + j) >> 3;
+            const int c = (col + j) >> 3;
             *reinterpret_cast<uint4*>(q_smem + r * (HD * 2) + ((c ^ (r & (CPR - 1))) << 4)) = w;
           }
         }
-        if (it.ranges > 1 && grp == 0) part_ml[(size_t)idx * BLOCK_M + r] = make_float2(m_final, l);
-        fence_before();
-      } else if (lane == 0) {
-        if (!*vabort) atomicExch(err, 113);
-        *vabort = 1;
       }
-      stop = softmax_bar_or(!ok || *vabort != 0);
-      if (!stop) {
-        const int ts = (int)threadIdx.x - 128;
-        const int c = ts % CPR;
-        if (it.ranges == 1) {
-          for (int row = ts / CPR; row < it.rows; row += 256 / CPR) {
-            const int node = row / plan.grp, g = row - node * plan.grp;
-            *reinterpret_cast<uint4*>(out + ((size_t)(it.q0 + it.node0 + node) * plan.nh + it.kvh * plan.grp + g) * HD + c * 8) =
-                *reinterpret_cast<const uint4*>(q_smem + row * (HD * 2) + ((c ^ (row & (CPR - 1))) << 4));
+      if (cut && tok >= 0 && half == 0) part_ml[(size_t)slot * BLOCK_M + r] = make_float2(m_run, l_all);
+      fence_before();
+      if (bad && tok >= 0) {
+        // the values that were taken out of V, to the rows that see them (every thread finishes what it wrote)
+#pragma unroll 1
+        for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += 8) {
+          float x[8] = {};
+#pragma unroll 1
+          for (int k = 0; k < TILE_N / 32 * seg.n_tiles; ++k) {
+            const int key0 = seg.tile_begin * TILE_N + 32 * k;
+            if (tile_masked(seg.r, plan, key0 & ~(TILE_N - 1)))
+              add_taken_out(x, sees32(seg.r, plan, tok, lo_row, key0), key0, seg.bt, plan, seg.kvh, v_cache, HD, d);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (x[e] == 0.0f) continue;
+            if (cut) {
+              float* at = reinterpret_cast<float*>(po + ((d + e) / 4) * BLOCK_M) + (e & 3);
+              *at += x[e];
+            } else {
+              bf16* at = reinterpret_cast<bf16*>(q_smem + r * (HD * 2) + (((d >> 3) ^ (r & (CPR - 1))) << 4)) + e;
+              *at = __float2bfloat16_rn(__bfloat162float(*at) + x[e]);
+            }
           }
         }
-        // what this warp read of O (tensor memory) and of the staged rows is in its registers or on its way out
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&epi_done);
       }
+      if (!cut) {
+        softmax_bar_or(false);
+        const int c = ts % CPR;
+        for (int row = ts / CPR; row < seg.rows; row += 256 / CPR) {
+          const int node = div_by(row, plan.inv_grp), h = row - node * plan.grp;
+          *reinterpret_cast<uint4*>(out + ((size_t)(seg.r.q0 + seg.node0 + node) * plan.nh + seg.kvh * plan.grp + h) * HD + c * 8) =
+              *reinterpret_cast<const uint4*>(q_smem + row * (HD * 2) + ((c ^ (row & (CPR - 1))) << 4));
+        }
+      } else if (!seg.began && ts == 0) {
+        // for the second kernel: the unit that this CTA's piece ends in, and how many pieces it is in
+        plan.cuts[blockIdx.x] = Cut{seg.r.q0 + seg.node0, seg.kvh, seg.rows, seg.pieces};
+      }
+      if (ts == 0) found_bad[(n_done + 1) & 1] = 0;   // last read between the barriers of the stretch before
+      // what this warp read of O (tensor memory) and of the staged rows is in its registers or on its way out
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&epi_done);
     }
   }
   fence_before();
@@ -628,39 +740,36 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) attn_tree_tc_kernel(
   }
 }
 
-// Joins the ranges of a row in order. A thread has one row and eight dims; rows are the fast index, as in the scratch.
+// Joins the pieces of the units that were cut, in order: block x the unit that begins in CTA x's piece and goes on behind it. A thread
+// has one row and eight dims; rows are the fast index, as in the scratch.
 template <int HD>
 __global__ void __launch_bounds__(BLOCK_M) attn_tree_tc_join_kernel(bf16* __restrict__ out, const float4* __restrict__ part_o,
-                                                                    const float2* __restrict__ part_ml,
-                                                                    const __grid_constant__ Plan plan) {
+                                                                    const float2* __restrict__ part_ml, const Cut* __restrict__ cuts,
+                                                                    int nh, int grp, unsigned inv_grp, int step) {
   pdl_wait();
   const int r = threadIdx.x, d8 = blockIdx.y;
-  const int m = blockIdx.x % plan.m_tiles, sh = blockIdx.x / plan.m_tiles;
-  const int kvh = sh % plan.nkv, s = sh / plan.nkv;
-  const int q0 = plan.cu_q[s], n = plan.cu_q[s + 1] - q0, node0 = m * plan.nodes_per_tile;
-  if (node0 >= n || r >= min(plan.nodes_per_tile, n - node0) * plan.grp) return;
-  const int kv_all = plan.seq_lens[s], kv_len = min(kv_all, plan.kv_cap);
-  if (kv_len <= 0) return;
-  const int ranges = cut_of(plan, kv_len, kv_all - n).ranges;
-  if (ranges == 1) return;
-  const size_t slot0 = (size_t)sh * plan.splits * plan.m_tiles + m;
+  const Cut cut = cuts[blockIdx.x];
+  if (cut.pieces < 2 || r >= cut.rows) return;
   float M = -INFINITY, L = 0.0f, acc[8] = {};
-  constexpr int U = 4;     // ranges in flight
-  for (int k0 = 0; k0 < ranges; k0 += U) {
+  constexpr int U = 4;     // pieces in flight
+  for (int k0 = 0; k0 < cut.pieces; k0 += U) {
     float2 ml[U];
     float4 a[U], b[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const size_t slot = slot0 + (size_t)min(k0 + k, ranges - 1) * plan.m_tiles;
-      const float4* po = part_o + (slot * (HD / 4) + d8 * 2) * BLOCK_M + r;
-      ml[k] = part_ml[slot * BLOCK_M + r];
-      a[k] = po[0];
-      b[k] = po[BLOCK_M];
+      ml[k] = make_float2(-INFINITY, 0.0f);
+      if (k0 + k < cut.pieces) {
+        const size_t at = (size_t)(2 * ((int)blockIdx.x + (k0 + k) * step) + (k0 + k == 0 ? 1 : 0)) * BLOCK_M;
+        const float4* po = part_o + at * (HD / 4) + d8 * 2 * BLOCK_M + r;
+        ml[k] = part_ml[at + r];
+        a[k] = po[0];
+        b[k] = po[BLOCK_M];
+      }
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      // a range of which the row sees nothing has neither weight nor maximum (but NaN scores have a sum without a maximum)
-      if (k0 + k >= ranges || (ml[k].x == -INFINITY && ml[k].y == 0.0f)) continue;
+      // a piece of which the row sees nothing has neither weight nor maximum (but NaN scores have a sum without a maximum)
+      if (k0 + k >= cut.pieces || (ml[k].x == -INFINITY && ml[k].y == 0.0f)) continue;
       const float mk = ml[k].x;
       const float m_new = fmaxf(M, mk);
       const float keep = M == m_new ? 1.0f : M == -INFINITY ? 0.0f : ex2_approx(M - m_new);
@@ -669,7 +778,7 @@ __global__ void __launch_bounds__(BLOCK_M) attn_tree_tc_join_kernel(bf16* __rest
       L = L * keep + ml[k].y * f;
       const float v[8] = {a[k].x, a[k].y, a[k].z, a[k].w, b[k].x, b[k].y, b[k].z, b[k].w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = keep == 1.0f ? fmaf(v[e], f, acc[e]) : fmaf(v[e], f, acc[e] * keep);
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(v[e], f, keep == 1.0f ? acc[e] : acc[e] * keep);
     }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -677,8 +786,8 @@ __global__ void __launch_bounds__(BLOCK_M) attn_tree_tc_join_kernel(bf16* __rest
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
 #pragma unroll
   for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  const int node = r / plan.grp, g = r - node * plan.grp;
-  *reinterpret_cast<uint4*>(out + ((size_t)(q0 + node0 + node) * plan.nh + kvh * plan.grp + g) * HD + d8 * 8) = w;
+  const int node = div_by(r, inv_grp), g = r - node * grp;
+  *reinterpret_cast<uint4*>(out + ((size_t)(cut.tok0 + node) * nh + cut.kvh * grp + g) * HD + d8 * 8) = w;
 }
 
 // Key tiles that a request of the batch looks at, at most.
@@ -691,67 +800,70 @@ int most_tiles(int max_q_len, int max_kv_len, int window) {
   return (int)(t < 1 ? 1 : t);
 }
 
+struct Sizes {
+  int grp, nodes, m_tiles, tiles, ctas, abreast;
+  long long cut_bytes, part_floats;      // the scratch: the cuts, then the pieces
+};
+// 0 if the kernel does not take these shapes
+bool sizes_of(Sizes& z, int S, int nh, int nkv, int hd, int page_size, int q_row_stride, float scale, int window, int max_q_len,
+              int max_kv_len) {
+  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv != 0 || nh / nkv > BLOCK_M || !(scale > 0.0f)) return false;
+  if (page_size < 8 || (page_size & (page_size - 1)) || (q_row_stride & 7) || S <= 0 || max_q_len <= 0 || max_kv_len <= 0) return false;
+  if (max_kv_len > MAX_KEYS || max_q_len > (1 << 24) || window < 0) return false;
+  z.grp = nh / nkv;
+  z.nodes = BLOCK_M / z.grp;
+  z.m_tiles = (max_q_len + z.nodes - 1) / z.nodes;
+  z.tiles = most_tiles(max_q_len, max_kv_len, window);
+  const double line = (double)S * nkv * z.m_tiles * z.tiles;
+  if (line > 1e9 || (double)S * nkv * z.m_tiles > 1e9) return false;
+  int sms = 1;
+  osb_num_sms(&sms);
+  const int most = CTAS_PER_SM * sms;
+  z.ctas = line < most ? (int)line : most;
+  z.abreast = S == 1 && z.m_tiles > 1 && z.m_tiles <= z.ctas ? z.m_tiles : 1;
+  z.cut_bytes = (long long)z.ctas * (long long)sizeof(Cut);
+  z.part_floats = z.tiles > 1 ? (long long)2 * z.ctas * BLOCK_M * (hd + 2) : 0;
+  return true;
+}
+
 template <int HD>
-int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, bf16* out, float* part_o, float* part_ml,
-           const bf16* v_cache, const Plan& plan, float scale_log2, int* err, cudaStream_t stream) {
-  // at least 120 KB so that one CTA is resident per SM: each takes all 512 tensor-memory columns
-  constexpr size_t need = (size_t)(HD / 64) * ATOM_BYTES * (1 + 2 * STAGES) + 1024;
-  constexpr size_t smem = need > 120 * 1024 ? need : 120 * 1024;
-  int sms = 0;
-  int rc = osb_allow_smem<attn_tree_tc_kernel<HD>>(smem);
-  if (rc == 0) rc = osb_num_sms(&sms);
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, bf16* out, float* part, const bf16* v_cache,
+           const Plan& plan, const Sizes& z, float scale_log2, cudaStream_t stream) {
+  int rc = osb_allow_smem<attn_tree_tc_kernel<HD>>(Layout<HD>::SMEM);
   if (rc) return rc;
-  rc = osb_launch(attn_tree_tc_kernel<HD>, dim3((unsigned)(plan.n_items < sms ? plan.n_items : sms)), dim3(NUM_THREADS), smem, stream, mq, mk, mv, out,
-                      (float4*)part_o, (float2*)part_ml, v_cache, plan, scale_log2, err);
-  if (rc == 0 && plan.splits > 1)
-    rc = osb_launch(attn_tree_tc_join_kernel<HD>, dim3((unsigned)(plan.S * plan.nkv * plan.m_tiles), HD / 8), dim3(BLOCK_M), 0, stream,
-                    out, (const float4*)part_o, (const float2*)part_ml, plan);
+  float4* po = (float4*)part;
+  float2* ml = (float2*)(part + (long long)2 * z.ctas * BLOCK_M * HD);
+  rc = osb_launch(attn_tree_tc_kernel<HD>, dim3((unsigned)z.ctas), dim3(NUM_THREADS), Layout<HD>::SMEM, stream, mq, mk, mv, out, po, ml,
+                  v_cache, plan, scale_log2);
+  if (rc == 0 && z.part_floats > 0)
+    rc = osb_launch(attn_tree_tc_join_kernel<HD>, dim3((unsigned)z.ctas, HD / 8), dim3(BLOCK_M), 0, stream, out, (const float4*)po,
+                    (const float2*)ml, (const Cut*)plan.cuts, plan.nh, plan.grp, plan.inv_grp, plan.abreast);
   return rc ? rc : osb_last_error();
 }
 }  // namespace
 
-// Into how many ranges (at most) a request's keys are cut, 0 if the kernel does not take the shapes. The cost of a cut in units of
-// one key tile: the waves of items over the SMs, each a range plus some 2 tiles for starting and ending it, and some 2 for the second
-// kernel; the smallest cut of the least cost.
-OSB_API int osb_attn_tree_tc_splits(int S, int nh, int nkv, int hd, int page_size, int q_row_stride, float scale, int window,
-                                    int max_q_len, int max_kv_len) {
-  if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv != 0 || nh / nkv > BLOCK_M || !(scale > 0.0f)) return 0;
-  if (page_size < 8 || (page_size & (page_size - 1)) || (q_row_stride & 7) || S <= 0 || max_q_len <= 0 || max_kv_len <= 0) return 0;
-  if (max_kv_len > MAX_KEYS || window < 0) return 0;
-  const int nodes = BLOCK_M / (nh / nkv);
-  const long long units = (long long)S * nkv * ((max_q_len + nodes - 1) / nodes);
-  if (units * MAX_TC_SPLITS > 2147483647LL) return 0;
-  const int tiles = most_tiles(max_q_len, max_kv_len, window);
-  int sms = 1;
-  osb_num_sms(&sms);
-  int best = 1;
-  long long best_cost = 0;
-  for (int s = 1; s <= MAX_TC_SPLITS && s <= tiles; ++s) {
-    const long long waves = (units * s + sms - 1) / sms;
-    const long long cost = waves * ((tiles + s - 1) / s + 2) + (s > 1 ? 2 : 0);
-    if (s == 1 || cost < best_cost) {
-      best = s;
-      best_cost = cost;
-    }
-  }
-  return best;
+// Bytes of scratch that osb_attn_tree_tc needs for these arguments, 0 if it does not take them.
+OSB_API long long osb_attn_tree_tc_scratch(int S, int nh, int nkv, int hd, int page_size, int q_row_stride, float scale, int window,
+                                           int max_q_len, int max_kv_len) {
+  Sizes z;
+  if (!sizes_of(z, S, nh, nkv, hd, page_size, q_row_stride, scale, window, max_q_len, max_kv_len)) return 0;
+  return z.cut_bytes + z.part_floats * 4;
 }
 
-// As osb_attn_tree for bf16 operands. splits: what osb_attn_tree_tc_splits gave for the same arguments (0 there: refused here with
-// OSB_ERR_UNSUPPORTED). With splits > 1: items = S x nkv x row tiles x splits, part_o items x 128 x hd and part_ml items x 256
-// floats, row tiles = ceil(max_q_len / (128 / (nh / nkv))).
+// As osb_attn_tree for bf16 operands; scratch: osb_attn_tree_tc_scratch bytes for the same arguments, on a 16-byte boundary. Shapes
+// for which that is 0 are refused with OSB_ERR_UNSUPPORTED.
 OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, const void* k_cache, const void* v_cache,
                              const int* block_table, int bt_stride, const int* cu_q, const int* seq_lens, const unsigned* mask,
                              int mask_words, const int* depth, int S, int nh, int nkv, int hd, int page_size, int num_pages,
-                             float scale, int window, int max_q_len, int max_kv_len, int splits, float* part_o, float* part_ml,
-                             int* err, cudaStream_t stream) {
+                             float scale, int window, int max_q_len, int max_kv_len, void* scratch, int* err,
+                             cudaStream_t stream) {
   if (S <= 0 || T <= 0 || max_q_len <= 0) return OSB_OK;
-  if (splits <= 0 || splits > MAX_TC_SPLITS || num_pages <= 0 ||
-      osb_attn_tree_tc_splits(S, nh, nkv, hd, page_size, q_row_stride, scale, window, max_q_len, max_kv_len) == 0)
+  Sizes z;
+  if (num_pages <= 0 || !sizes_of(z, S, nh, nkv, hd, page_size, q_row_stride, scale, window, max_q_len, max_kv_len))
     return OSB_ERR_UNSUPPORTED;
   if (((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15))
     return OSB_ERR_UNSUPPORTED;
-  if ((window > 0 && depth == nullptr) || (splits > 1 && (part_o == nullptr || part_ml == nullptr))) return OSB_ERR_BAD_SHAPE;
+  if ((window > 0 && depth == nullptr) || scratch == nullptr || ((uintptr_t)scratch & 15)) return OSB_ERR_BAD_SHAPE;
   Plan p = {};
   p.block_table = block_table;
   p.cu_q = cu_q;
@@ -759,23 +871,24 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   p.mask = mask;
   p.depth = depth;
   p.err = err;
+  p.cuts = (Cut*)scratch;
   p.bt_stride = bt_stride;
   p.mask_words = mask_words;
   p.S = S;
   p.nh = nh;
   p.nkv = nkv;
-  p.grp = nh / nkv;
+  p.grp = z.grp;
   while ((1 << p.log2ps) < page_size) ++p.log2ps;
   p.num_pages = num_pages;
   p.window = window;
   p.max_q_len = max_q_len;
   const long long table = (long long)bt_stride * page_size;     // keys behind the block table cannot be read
   p.kv_cap = table < max_kv_len ? (int)table : max_kv_len;
-  p.nodes_per_tile = BLOCK_M / p.grp;
-  p.m_tiles = (max_q_len + p.nodes_per_tile - 1) / p.nodes_per_tile;
-  p.splits = splits;
-  p.chunk_tiles = (most_tiles(max_q_len, max_kv_len, window) + splits - 1) / splits;
-  p.n_items = S * nkv * p.m_tiles * splits;
+  p.nodes_per_tile = z.nodes;
+  p.m_tiles = z.m_tiles;
+  p.abreast = z.abreast;
+  p.inv_nodes = z.nodes == 1 ? 0u : (unsigned)((0x100000000ull + z.nodes - 1) / z.nodes);
+  p.inv_grp = z.grp == 1 ? 0u : (unsigned)((0x100000000ull + z.grp - 1) / z.grp);
   CUtensorMap mq, mk, mv;
   {
     const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nh, (cuuint64_t)T};
@@ -788,14 +901,14 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
     const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)page_size, (cuuint64_t)nkv, (cuuint64_t)num_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)page_size * hd * 2,
                                    (cuuint64_t)nkv * page_size * hd * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(page_size < 128 ? page_size : 128), 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(page_size < TILE_N ? page_size : TILE_N), 1, 1};
     int rc = make_map_bf16(&mk, k_cache, 4, dims, strides, box);
     if (rc) return rc;
     rc = make_map_bf16(&mv, v_cache, 4, dims, strides, box);
     if (rc) return rc;
   }
+  float* part = (float*)((unsigned char*)scratch + z.cut_bytes);
   const float scale_log2 = scale * LOG2E;
-  if (hd == 64)
-    return launch<64>(mq, mk, mv, (bf16*)out, part_o, part_ml, (const bf16*)v_cache, p, scale_log2, err, stream);
-  return launch<128>(mq, mk, mv, (bf16*)out, part_o, part_ml, (const bf16*)v_cache, p, scale_log2, err, stream);
+  if (hd == 64) return launch<64>(mq, mk, mv, (bf16*)out, part, (const bf16*)v_cache, p, z, scale_log2, stream);
+  return launch<128>(mq, mk, mv, (bf16*)out, part, (const bf16*)v_cache, p, z, scale_log2, stream);
 }

@@ -29,9 +29,9 @@ _SIGNATURES = {
     "osb_attn_tree_splits": [_INT],
     "osb_attn_tree": [_PTR, _INT, _PTR, _INT, _INT, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT,
                       _INT, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR],
-    "osb_attn_tree_tc_splits": [_INT, _INT, _INT, _INT, _INT, _INT, _FLOAT, _INT, _INT, _INT],
+    "osb_attn_tree_tc_scratch": [_INT, _INT, _INT, _INT, _INT, _INT, _FLOAT, _INT, _INT, _INT],
     "osb_attn_tree_tc": [_PTR, _PTR, _INT, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT, _INT, _INT,
-                         _FLOAT, _INT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR],
+                         _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR],
     "osb_verify_drafts": [_PTR] * 11 + [_INT] * 5 + [_PTR, _PTR],
     "osb_compact_cache": [_PTR, _INT, _INT, _INT, _INT, _INT, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR],
     "osb_copy_pages": [_PTR, _LONG, _INT, _INT, _PTR, _PTR, _INT, _PTR],
@@ -43,6 +43,7 @@ def declare(lib: ctypes.CDLL) -> None:
     where a step's launches take a few microseconds, and an object per address costs about as much."""
     for name, types in _SIGNATURES.items():
         getattr(lib, name).argtypes = types
+    lib.osb_attn_tree_tc_scratch.restype = _LONG
 
 
 def _on_device(ref: torch.Tensor) -> int:
@@ -158,22 +159,17 @@ class SpeculativeOps:
         qp, kp, vp, op = qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
         dp = depth.data_ptr() if depth is not None else None
         err = self.err_flag(qkv.device).data_ptr()
-        splits = 0
+        need = 0
         if (not exact and qkv.dtype is _BF16 and k_cache.dtype is _BF16 and out_dtype is _BF16 and (qp | kp | vp | op) % 16 == 0):
-            splits = self.lib.osb_attn_tree_tc_splits(S, nh, nkv, hd, page_size, width, scale, win, max_q_len, max_kv_len)
-        if splits > 0:
-            # rows of a row tile's ranges, then (maximum, sum) of each
-            part = ml = None
-            if splits > 1:
-                slots = S * nkv * -(-max_q_len // (128 // (nh // nkv))) * splits * 128
-                scratch = torch.empty(slots * (hd + 2), dtype=_F32, device=qkv.device)
-                part = scratch.data_ptr()
-                ml = part + 4 * slots * hd
+            need = self.lib.osb_attn_tree_tc_scratch(S, nh, nkv, hd, page_size, width, scale, win, max_q_len, max_kv_len)
+        if need > 0:
+            scratch = torch.empty(need, dtype=torch.uint8, device=qkv.device)
             rc = self.lib.osb_attn_tree_tc(
                 op, qp, width, T, kp, vp, block_table.data_ptr(), bt_width, cu_q.data_ptr(), seq_lens.data_ptr(),
-                tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len, max_kv_len, splits, part,
-                ml, err, self._raw_stream(dev))
+                tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len, max_kv_len,
+                scratch.data_ptr(), err, self._raw_stream(dev))
             self._ok(rc, "attn_tree_tc")
+            self.launches += 1 if max_kv_len > 64 else 0
         else:
             splits = self.lib.osb_attn_tree_splits(max_kv_len)
             part = ml = None
@@ -186,7 +182,7 @@ class SpeculativeOps:
                 seq_lens.data_ptr(), tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len,
                 max_kv_len, part, ml, err, self._raw_stream(dev))
             self._ok(rc, "attn_tree")
-        self.launches += 1 if splits > 1 else 0
+            self.launches += 1 if splits > 1 else 0
         return out
 
     # ------------------------------------------------------------------ verification
