@@ -26,9 +26,9 @@ _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
 _PTR, _INT, _FLOAT, _LONG = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 _SIGNATURES = {
-    "osb_attn_tree_splits": [_INT],
+    "osb_attn_tree_scratch": [_INT, _INT, _INT, _INT, _INT, _INT],
     "osb_attn_tree": [_PTR, _INT, _PTR, _INT, _INT, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT,
-                      _INT, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR, _PTR],
+                      _INT, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR],
     "osb_attn_tree_tc_scratch": [_INT, _INT, _INT, _INT, _INT, _INT, _FLOAT, _INT, _INT, _INT],
     "osb_attn_tree_tc": [_PTR, _PTR, _INT, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT, _INT, _INT,
                          _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR],
@@ -43,7 +43,7 @@ def declare(lib: ctypes.CDLL) -> None:
     where a step's launches take a few microseconds, and an object per address costs about as much."""
     for name, types in _SIGNATURES.items():
         getattr(lib, name).argtypes = types
-    lib.osb_attn_tree_tc_scratch.restype = _LONG
+    lib.osb_attn_tree_scratch.restype = lib.osb_attn_tree_tc_scratch.restype = _LONG
 
 
 def _on_device(ref: torch.Tensor) -> int:
@@ -171,18 +171,14 @@ class SpeculativeOps:
             self._ok(rc, "attn_tree_tc")
             self.launches += 1 if max_kv_len > 64 else 0
         else:
-            splits = self.lib.osb_attn_tree_splits(max_kv_len)
-            part = ml = None
-            if splits > 1:
-                scratch = torch.empty(T * nh * splits * (hd + 2), dtype=_F32, device=qkv.device)
-                part = scratch.data_ptr()
-                ml = part + 4 * T * nh * splits * hd
+            need = self.lib.osb_attn_tree_scratch(S, nh, nkv, hd, max_q_len, max_kv_len)
+            scratch = torch.empty(need, dtype=_F32, device=qkv.device) if need > 0 else None
             rc = self.lib.osb_attn_tree(
                 op, _dt(out), qp, _dt(qkv), width, kp, vp, _dt(k_cache), block_table.data_ptr(), bt_width, cu_q.data_ptr(),
                 seq_lens.data_ptr(), tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len,
-                max_kv_len, part, ml, err, self._raw_stream(dev))
+                max_kv_len, scratch.data_ptr() if need > 0 else None, err, self._raw_stream(dev))
             self._ok(rc, "attn_tree")
-            self.launches += 1 if splits > 1 else 0
+            self.launches += 1 if need > 0 else 0
         return out
 
     # ------------------------------------------------------------------ verification

@@ -224,7 +224,7 @@ def tree_args(**over):
     a.update(over)
     o, q, c = a["dtypes"]
     return (NULL, o, NULL, q, 512, NULL, NULL, c, NULL, 4, NULL, NULL, NULL, 1, a["depth"], a["S"], a["nh"], a["nkv"], a["hd"],
-            a["page"], a["pages"], ctypes.c_float(1.0), a["window"], a["max_q"], a["max_kv"], a["part"], a["part"], NULL, NULL)
+            a["page"], a["pages"], ctypes.c_float(1.0), a["window"], a["max_q"], a["max_kv"], a["part"], NULL, NULL)
 
 
 @pytest.mark.parametrize("over,status", [
@@ -235,10 +235,24 @@ def test_tree_attention_entry_refuses(over, status):
     assert library.load().osb_attn_tree(*tree_args(**over)) == status
 
 
-def test_ranges_of_the_tree_attention_hold_for_every_shorter_request():
-    f = library.load().osb_attn_tree_splits
-    got = [f(n) for n in (-5, 0, 1, 256, 257, 8192, 8193, 100000, 2**31 - 1)]
-    assert got == [1, 1, 1, 1, 2, 32, 32, 32, 32] and got == sorted(got)
+def test_scratch_of_the_32_bit_tree_attention_holds_every_smaller_request():
+    """A request's rows x ranges never need more than what the largest request of its batch was given."""
+    f = library.load().osb_attn_tree_scratch
+    f.restype = ctypes.c_longlong
+    assert f(1, 4, 2, 64, 8, 64) == 0 and f(0, 4, 2, 64, 8, 640) == 0
+
+    def ranges(kv, rows):      # as the kernel cuts
+        most = max(1, 128 // -(-rows // 32))
+        per = -(-kv // most)
+        return -(-kv // (-(-per // 64) * 64))
+
+    for max_q, grp, max_kv in [(1, 1, 65), (3, 6, 700), (24, 6, 1000), (64, 8, 5000), (300, 8, 4097), (9, 4, 100000)]:
+        cap = (f(1, grp, 1, 62, max_q, max_kv) - 1) // 64
+        for q in sorted({1, 2, max_q // 3 + 1, max_q}):
+            for kv in sorted({1, 64, 65, 128, max_kv // 2, 4096, 4100, max_kv - 1, max_kv}):
+                if kv <= max_kv and q <= max_q and ranges(kv, q * grp) > 1:      # (one range goes straight to the output)
+                    assert q * grp * ranges(kv, q * grp) <= cap, (max_q, grp, max_kv, q, kv)
+                    assert ranges(kv, q * grp) <= ranges(min(max_kv, 8192), 1)
 
 
 def verify_args(**over):
