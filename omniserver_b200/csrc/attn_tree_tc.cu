@@ -42,9 +42,9 @@ constexpr int MIN_PIECE = 2;                         // key tiles of a CTA at le
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 
-// A unit that was cut, by the CTA in which it begins: its first token, kv head, rows and number of pieces (0: no such unit).
+// A unit (request, kv head, row tile): the CTA in whose piece it begins, and into how many pieces it was cut.
 struct Cut {
-  int tok0, kvh, rows, pieces;
+  int cta, pieces;
 };
 
 // The step, the same for every CTA.
@@ -55,9 +55,9 @@ struct Plan {
   const unsigned* mask;
   const int* depth;
   int* err;
-  Cut* cuts;           // scratch, by CTA
+  Cut* cuts;           // scratch, by unit: (request x kv heads + head) x row tiles + tile
   int bt_stride, mask_words, S, nh, nkv, grp, log2ps, num_pages, window, max_q_len, kv_cap;
-  int nodes_per_tile, m_tiles;
+  int nodes_per_tile, m_tiles, ctas;
   int abreast;                      // row tiles that neighbouring CTAs take at the same time (1: row tiles are units like others)
   unsigned inv_nodes, inv_grp;      // 2^32 / nodes_per_tile and / grp, rounded up
 };
@@ -98,7 +98,7 @@ struct Seg {
   int kvh, node0, rows;         // the row tile: its first node, its number of rows
   int tile_begin, n_tiles;
   bool whole, began;            // whole: all the unit's tiles; began: the unit began in an earlier piece
-  int pieces;                   // of a unit that begins here and is cut
+  int unit, pieces;             // the unit's number; into how many pieces it is cut, if it begins here
   const int* bt;
 };
 
@@ -125,7 +125,8 @@ struct Walk {
     seg.tile_begin = r.first_tile + t0;
     seg.whole = seg.n_tiles == r.tiles;
     seg.began = t0 > 0;
-    seg.pieces = 1 + (r.tiles - seg.n_tiles + piece - 1) / piece;
+    seg.unit = (s * p.nkv + seg.kvh) * p.m_tiles + (p.abreast > 1 ? m : unit - seg.kvh * units);
+    seg.pieces = 1 + (seg.whole ? 0 : (r.tiles - seg.n_tiles + piece - 1) / piece);
     seg.bt = p.block_table + (size_t)s * p.bt_stride;
     g += seg.n_tiles;
     return true;
@@ -352,7 +353,6 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       run += chunk;
     }
   }
-  if (tid == 128) plan.cuts[blockIdx.x].pieces = 0;      // (the thread that may say otherwise later)
   fence_before();
   __syncthreads();
   fence_after();
@@ -721,10 +721,8 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
           *reinterpret_cast<uint4*>(out + ((size_t)(seg.r.q0 + seg.node0 + node) * plan.nh + seg.kvh * plan.grp + h) * HD + c * 8) =
               *reinterpret_cast<const uint4*>(q_smem + row * (HD * 2) + ((c ^ (row & (CPR - 1))) << 4));
         }
-      } else if (!seg.began && ts == 0) {
-        // for the second kernel: the unit that this CTA's piece ends in, and how many pieces it is in
-        plan.cuts[blockIdx.x] = Cut{seg.r.q0 + seg.node0, seg.kvh, seg.rows, seg.pieces};
       }
+      if (!seg.began && ts == 0) plan.cuts[seg.unit] = Cut{(int)blockIdx.x, seg.pieces};     // for the second kernel
       if (ts == 0) found_bad[(n_done + 1) & 1] = 0;   // last read between the barriers of the stretch before
       // what this warp read of O (tensor memory) and of the staged rows is in its registers or on its way out
       fence_async_smem();
@@ -740,54 +738,91 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   }
 }
 
-// Joins the pieces of the units that were cut, in order: block x the unit that begins in CTA x's piece and goes on behind it. A thread
-// has one row and eight dims; rows are the fast index, as in the scratch.
-template <int HD>
-__global__ void __launch_bounds__(BLOCK_M) attn_tree_tc_join_kernel(bf16* __restrict__ out, const float4* __restrict__ part_o,
-                                                                    const float2* __restrict__ part_ml, const Cut* __restrict__ cuts,
-                                                                    int nh, int grp, unsigned inv_grp, int step) {
+// Joins the pieces of the units that were cut. A warp has 32 rows (the fast index, as in the scratch), DIMS dims and every WARPS-th
+// piece, all its loads in flight at once where they fit; the WARPS warps of the same rows then join what they have, in order. What it
+// takes is three round trips to the L2, if all warps are on the SMs at once: few units in many pieces take many warps with few
+// dims each, many units in two or three pieces one warp per 32 rows and 32 dims.
+template <int HD, int DIMS, int WARPS>
+__global__ void __launch_bounds__(256, DIMS == 32 ? 2 : 3) attn_tree_tc_join_kernel(bf16* __restrict__ out, const float4* __restrict__ part_o,
+                                                                   const float2* __restrict__ part_ml,
+                                                                   const __grid_constant__ Plan plan) {
+  constexpr int Q = DIMS / 4, U = DIMS == 8 ? 4 : 2;     // U: pieces of a warp in flight
+  __shared__ float2 sh_ml[8][32];
+  __shared__ float4 sh_o[8][Q][32];
   pdl_wait();
-  const int r = threadIdx.x, d8 = blockIdx.y;
-  const Cut cut = cuts[blockIdx.x];
-  if (cut.pieces < 2 || r >= cut.rows) return;
-  float M = -INFINITY, L = 0.0f, acc[8] = {};
-  constexpr int U = 4;     // pieces in flight
-  for (int k0 = 0; k0 < cut.pieces; k0 += U) {
-    float2 ml[U];
-    float4 a[U], b[U];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % WARPS;
+  const int group = (int)blockIdx.y * (8 / WARPS) + warp / WARPS, block = group / (HD / DIMS);
+  const int unit = blockIdx.x, sh = unit / plan.m_tiles, m = unit - sh * plan.m_tiles;
+  const int s = sh / plan.nkv, kvh = sh - s * plan.nkv;
+  const Cut cut = plan.cuts[unit];                       // (not written where there is no such unit)
+  const Req q = req_of(plan, s);
+  const int node0 = m * plan.nodes_per_tile, step = plan.abreast;
+  if (q.tiles <= 0 || m >= q.m_tiles || cut.pieces < 2) return;
+  // (a CTA that gave up in a wait wrote no cut: what stands there instead must not lead out of the scratch)
+  if (cut.cta < 0 || cut.cta >= plan.ctas || cut.pieces > (plan.ctas - cut.cta + step - 1) / step) return;
+  const int rows = min(plan.nodes_per_tile, q.n - node0) * plan.grp;
+  const int r = block * 32 + lane, d0 = (group - block * (HD / DIMS)) * DIMS;
+  float M = -INFINITY, L = 0.0f, acc[DIMS] = {};
+  // a piece of which the row sees nothing has neither weight nor maximum (but NaN scores have a sum without a maximum)
+  auto take = [&](float2 ml, const float4 (&o)[Q]) {
+    if (ml.x == -INFINITY && ml.y == 0.0f) return;
+    const float m_new = fmaxf(M, ml.x);
+    const float keep = M == m_new ? 1.0f : M == -INFINITY ? 0.0f : ex2_approx(M - m_new);
+    const float f = ml.x == m_new ? 1.0f : ex2_approx(ml.x - m_new);
+    M = m_new;
+    L = L * keep + ml.y * f;
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.0f);
-      if (k0 + k < cut.pieces) {
-        const size_t at = (size_t)(2 * ((int)blockIdx.x + (k0 + k) * step) + (k0 + k == 0 ? 1 : 0)) * BLOCK_M;
-        const float4* po = part_o + at * (HD / 4) + d8 * 2 * BLOCK_M + r;
-        ml[k] = part_ml[at + r];
-        a[k] = po[0];
-        b[k] = po[BLOCK_M];
+    for (int k = 0; k < Q; ++k) {
+      const float v[4] = {o[k].x, o[k].y, o[k].z, o[k].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * k + e] = fmaf(v[e], f, keep == 1.0f ? acc[4 * k + e] : acc[4 * k + e] * keep);
+    }
+  };
+  if (r < rows)
+    for (int k0 = mine; k0 < cut.pieces; k0 += WARPS * U) {
+      float2 ml[U];
+      float4 o[U][Q];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int piece = k0 + WARPS * k;
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        if (piece < cut.pieces) {
+          const size_t at = (size_t)(2 * (cut.cta + piece * step) + (piece == 0 ? 1 : 0)) * BLOCK_M;
+          const float4* po = part_o + at * (HD / 4) + (d0 / 4) * BLOCK_M + r;
+          ml[k] = part_ml[at + r];
+#pragma unroll
+          for (int e = 0; e < Q; ++e) o[k][e] = po[e * BLOCK_M];
+        }
       }
-    }
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      // a piece of which the row sees nothing has neither weight nor maximum (but NaN scores have a sum without a maximum)
-      if (k0 + k >= cut.pieces || (ml[k].x == -INFINITY && ml[k].y == 0.0f)) continue;
-      const float mk = ml[k].x;
-      const float m_new = fmaxf(M, mk);
-      const float keep = M == m_new ? 1.0f : M == -INFINITY ? 0.0f : ex2_approx(M - m_new);
-      const float f = mk == m_new ? 1.0f : ex2_approx(mk - m_new);
-      M = m_new;
-      L = L * keep + ml[k].y * f;
-      const float v[8] = {a[k].x, a[k].y, a[k].z, a[k].w, b[k].x, b[k].y, b[k].z, b[k].w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(v[e], f, keep == 1.0f ? acc[e] : acc[e] * keep);
+      for (int k = 0; k < U; ++k)
+        if (k0 + WARPS * k < cut.pieces) take(ml[k], o[k]);
     }
+  if (mine > 0) {
+    sh_ml[warp][lane] = make_float2(M, L);
+#pragma unroll
+    for (int e = 0; e < Q; ++e) sh_o[warp][e][lane] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+  }
+  __syncthreads();
+  if (mine > 0 || r >= rows) return;
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) {
+    float4 o[Q];
+#pragma unroll
+    for (int e = 0; e < Q; ++e) o[e] = sh_o[warp + w][e][lane];
+    take(sh_ml[warp + w][lane], o);
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  uint4 w;
-  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+  const int node = div_by(r, plan.inv_grp), g = r - node * plan.grp;
+  bf16* to = out + ((size_t)(q.q0 + node0 + node) * plan.nh + kvh * plan.grp + g) * HD + d0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  const int node = div_by(r, inv_grp), g = r - node * grp;
-  *reinterpret_cast<uint4*>(out + ((size_t)(cut.tok0 + node) * nh + cut.kvh * grp + g) * HD + d8 * 8) = w;
+  for (int d = 0; d < DIMS; d += 8) {
+    uint4 w;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(acc[d + 2 * e] * inv, acc[d + 2 * e + 1] * inv);
+    *reinterpret_cast<uint4*>(to + d) = w;
+  }
 }
 
 // Key tiles that a request of the batch looks at, at most.
@@ -801,7 +836,7 @@ int most_tiles(int max_q_len, int max_kv_len, int window) {
 }
 
 struct Sizes {
-  int grp, nodes, m_tiles, tiles, ctas, abreast;
+  int grp, nodes, m_tiles, row_blocks, tiles, ctas, abreast;
   long long cut_bytes, part_floats;      // the scratch: the cuts, then the pieces
 };
 // 0 if the kernel does not take these shapes
@@ -813,6 +848,7 @@ bool sizes_of(Sizes& z, int S, int nh, int nkv, int hd, int page_size, int q_row
   z.grp = nh / nkv;
   z.nodes = BLOCK_M / z.grp;
   z.m_tiles = (max_q_len + z.nodes - 1) / z.nodes;
+  z.row_blocks = ((max_q_len < z.nodes ? max_q_len : z.nodes) * z.grp + 31) / 32;
   z.tiles = most_tiles(max_q_len, max_kv_len, window);
   const double line = (double)S * nkv * z.m_tiles * z.tiles;
   if (line > 1e9 || (double)S * nkv * z.m_tiles > 1e9) return false;
@@ -821,7 +857,7 @@ bool sizes_of(Sizes& z, int S, int nh, int nkv, int hd, int page_size, int q_row
   const int most = CTAS_PER_SM * sms;
   z.ctas = line < most ? (int)line : most;
   z.abreast = S == 1 && z.m_tiles > 1 && z.m_tiles <= z.ctas ? z.m_tiles : 1;
-  z.cut_bytes = (long long)z.ctas * (long long)sizeof(Cut);
+  z.cut_bytes = ((long long)S * nkv * z.m_tiles * (long long)sizeof(Cut) + 15) / 16 * 16;
   z.part_floats = z.tiles > 1 ? (long long)2 * z.ctas * BLOCK_M * (hd + 2) : 0;
   return true;
 }
@@ -835,9 +871,22 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   float2* ml = (float2*)(part + (long long)2 * z.ctas * BLOCK_M * HD);
   rc = osb_launch(attn_tree_tc_kernel<HD>, dim3((unsigned)z.ctas), dim3(NUM_THREADS), Layout<HD>::SMEM, stream, mq, mk, mv, out, po, ml,
                   v_cache, plan, scale_log2);
-  if (rc == 0 && z.part_floats > 0)
-    rc = osb_launch(attn_tree_tc_join_kernel<HD>, dim3((unsigned)z.ctas, HD / 8), dim3(BLOCK_M), 0, stream, out, (const float4*)po,
-                    (const float2*)ml, (const Cut*)plan.cuts, plan.nh, plan.grp, plan.inv_grp, plan.abreast);
+  if (rc == 0 && z.part_floats > 0) {
+    const int units = plan.S * plan.nkv * plan.m_tiles;
+    // warps for so many dims each and so many sharing the pieces of a row: as many as make about one wave. Both kernels with each
+    // of the four, in this order, us: one request of 2,048 keys on 2 kv heads 13.7, 14.7, 15.7, 20.3; 8 ragged ones of up to 4,096
+    // on 4 kv heads 41.8, 31.0, 29.5, 31.0; 64 of 2,100 79.7, 56.3, 51.8, 50.7
+    const long long groups = (long long)units * z.row_blocks, wave = 12LL * z.ctas;
+    auto join = [&](auto k, int dims, int warps) {
+      const int per_unit = z.row_blocks * (HD / dims), per_cta = 8 / warps;
+      return osb_launch(k, dim3((unsigned)units, (unsigned)((per_unit + per_cta - 1) / per_cta)), dim3(256), 0, stream, out,
+                        (const float4*)po, (const float2*)ml, plan);
+    };
+    if (groups * (HD / 8) * 8 <= wave) rc = join(attn_tree_tc_join_kernel<HD, 8, 8>, 8, 8);
+    else if (groups * (HD / 16) * 4 <= wave) rc = join(attn_tree_tc_join_kernel<HD, 16, 4>, 16, 4);
+    else if (groups * (HD / 16) * 2 <= wave / 3 * 4) rc = join(attn_tree_tc_join_kernel<HD, 16, 2>, 16, 2);
+    else rc = join(attn_tree_tc_join_kernel<HD, 32, 1>, 32, 1);
+  }
   return rc ? rc : osb_last_error();
 }
 }  // namespace
@@ -886,6 +935,7 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   p.kv_cap = table < max_kv_len ? (int)table : max_kv_len;
   p.nodes_per_tile = z.nodes;
   p.m_tiles = z.m_tiles;
+  p.ctas = z.ctas;
   p.abreast = z.abreast;
   p.inv_nodes = z.nodes == 1 ? 0u : (unsigned)((0x100000000ull + z.nodes - 1) / z.nodes);
   p.inv_grp = z.grp == 1 ? 0u : (unsigned)((0x100000000ull + z.grp - 1) / z.grp);

@@ -660,3 +660,330 @@ def test_copy_pages_refuses():
     with pytest.raises(KernelError, match="CUDA tensor"):
         K().copy_pages(cache.cpu(), [0], [1])
     assert torch.equal(cache, before)
+
+
+# ------------------------------------------------------------------ streams, graphs, devices, and a step as a whole
+def device_step(step):
+    d = {n: getattr(step, n).to(DEV) for n in ("qkv", "k", "v", "bt", "cu", "lens", "mask", "depth")}
+
+    def call(out=None):
+        return K().tree_attention(d["qkv"], d["k"], d["v"], d["bt"], d["cu"], d["lens"], d["mask"], step.nh, step.nkv, step.hd,
+                                  step.hd ** -0.5, None, max(step.q_lens), max(int(x) for x in step.lens), step.qkv.dtype, out=out)
+    return d, call
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tree_attention_on_two_streams_at_once(dtype):
+    """Calls on two streams, interleaved, share nothing: each gives what it gives alone."""
+    big = device_step(Step([40, 9, 17], [2500, 700, 30], 12, 2, 128, 32, dtype, seed=1))[1]
+    small = device_step(Step([5, 1], [300, 900], 12, 2, 128, 32, dtype, seed=2))[1]
+    want = big(), small()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, f in enumerate((big, small)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(f())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+    K().check_device_errors()
+
+
+def test_verify_on_two_streams_at_once():
+    calls, want = [], []
+    for seed, q_lens in ((1, [9, 4, 30]), (2, [6])):
+        args, q = drafts(q_lens, 30000, seed=seed, dense=True)
+        dev = {n: t.to(DEV) for n, t in args.items()}
+        temp, qd = torch.full((len(q_lens),), 0.9, device=DEV), q.to(DEV)
+        calls.append(lambda dev=dev, temp=temp, qd=qd, n=max(q_lens): K().verify_drafts(**dev, max_q_len=n, max_depth=5, temperature=temp, draft_probs=qd))
+        want.append([t.clone() for t in calls[-1]()])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for g in got[i] for a, b in zip(g, want[i]))
+    K().check_device_errors()
+
+
+def test_captured_calls_replay_with_new_data():
+    """Two graphs of the calls, captured one after the other, replayed in turn with other lengths, masks, logits and paths in the
+    same buffers."""
+    steps = [Step([20, 7, 3], b, 12, 2, 128, 32, BF16, seed=5) for b in ([900, 40, 333], [10, 500, 800], [0, 1000, 64])]
+    # one pool of pages and one width of table for all of them
+    pages, width = max(s.k.shape[0] for s in steps), max(s.bt.shape[1] for s in steps)
+    k, v = torch.zeros(pages, 2, 32, 128, dtype=BF16, device=DEV), torch.zeros(pages, 2, 32, 128, dtype=BF16, device=DEV)
+    bt = torch.full((3, width), -1, dtype=torch.int32, device=DEV)
+    qkv, mask, lens, cu = steps[0].qkv.to(DEV), steps[0].mask.to(DEV), steps[0].lens.to(DEV), steps[0].cu.to(DEV)
+    args, _ = drafts([20, 7, 3], 5000, seed=1)
+    dev = {n: t.to(DEV) for n, t in args.items()}
+    temp = torch.ones(3, device=DEV)
+    cache = torch.zeros(2, 2, pages, 2, 32, 128, dtype=BF16, device=DEV)
+
+    def whole():
+        o = K().tree_attention(qkv, k, v, bt, cu, lens, mask, 12, 2, 128, 0.09, None, 20, 1100, BF16)
+        new, path, count = K().verify_drafts(**dev, max_q_len=20, max_depth=6, temperature=temp)
+        K().compact_cache(cache, bt, cu, lens, path, count)
+        return o, new, path, count
+
+    def load(i):
+        s = steps[i]
+        for dst, src in ((qkv, s.qkv), (mask, s.mask), (lens, s.lens)):
+            dst.copy_(src)
+        k.zero_()[:s.k.shape[0]].copy_(s.k)
+        v.zero_()[:s.v.shape[0]].copy_(s.v)
+        bt.fill_(-1)[:, :s.bt.shape[1]].copy_(s.bt)
+        other, _ = drafts([20, 7, 3], 5000, seed=10 + i)
+        for n, t in other.items():
+            dev[n].copy_(t)
+        cache.copy_(torch.randn(cache.shape, generator=torch.Generator().manual_seed(i)))
+
+    load(0)
+    whole()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(whole())
+        graphs.append(g)
+    for i in (1, 0, 2, 1):
+        for g, o in zip(graphs, outs):
+            load(i)
+            g.replay()
+            got = [t.clone() for t in o] + [cache.clone()]
+            load(i)
+            want = list(whole()) + [cache]
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+    K().check_device_errors()
+
+
+def test_tensors_have_to_be_on_the_current_device(monkeypatch):
+    """(Shown with a device number that is not this one's: the tests run on one GPU.)"""
+    from omniserver_b200.ops import KernelError
+    s = Step([5], [30], 4, 2, 64, 16, F32)
+    d, call = device_step(s)
+    call()
+    cache = torch.zeros(1, 2, 4, 2, 8, 16, device=DEV)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 5)
+    with pytest.raises(KernelError, match="not the current device"):
+        call()
+    with pytest.raises(KernelError, match="not the current device"):
+        K().copy_pages(cache, [0], [1])
+    with pytest.raises(KernelError, match="not the current device"):
+        K().verify_drafts(torch.zeros(1, 4, device=DEV), d["cu"][:1], d["cu"][:1], d["cu"], torch.zeros(1, device=DEV), 1, 1)
+
+
+def test_empty_batches():
+    z = torch.zeros(0, dtype=torch.int32, device=DEV)
+    one = torch.zeros(1, dtype=torch.int32, device=DEV)
+    k = torch.zeros(3, 2, 16, 64, dtype=BF16, device=DEV)
+    out = K().tree_attention(torch.zeros(0, 512, dtype=BF16, device=DEV), k, k, z.view(0, 4), one, z, z.view(0, 1), 4, 2, 64, 1.0, None, 0, 0, BF16)
+    assert out.shape == (0, 256)
+    new, path, count = K().verify_drafts(torch.zeros(0, 7, device=DEV), z, z, one, torch.zeros(0, device=DEV), 0, 2)
+    assert new.shape == (0, 3) and path.shape == (0, 3) and count.shape == (0,)
+    K().compact_cache(torch.zeros(1, 2, 3, 2, 16, 64, device=DEV), z.view(0, 4), one, z, z.view(0, 3), z)
+    K().check_device_errors()
+
+
+def test_many_requests_in_one_step():
+    """More requests than a CTA has threads: the line of tiles is laid out in several rounds."""
+    rng = np.random.default_rng(3)
+    q_lens, bases = rng.integers(0, 4, 900).tolist(), rng.integers(0, 40, 900).tolist()
+    for dtype in (BF16, F32):
+        step = Step(q_lens, bases, 2, 1, 64, 16, dtype, seed=3)
+        check(step, step.got(), *step.want(), runs_on_tensor_cores(step))
+
+
+def test_fork_then_both_go_on():
+    """A forked request's cache is its parent's until they go on; then neither sees the other."""
+    from omniserver_b200.cache import CacheManager
+    from omniserver_b200.models.decoder import EntryNeeds
+    from omniserver_b200.parts.base import KVCacheNeed
+    m = CacheManager([EntryNeeds(KVCacheNeed(2, 64, None), [], None)] * 3, [], 16, 12, 4, BF16, DEV)
+    st = m.groups[0].storage
+    m.begin("a")
+    m.reserve("a", 37)
+    slots = torch.from_numpy(m.slot_map(0, ["a"], [37])).long()
+    m.commit("a", 37)
+    st[:, :, slots // 16, :, slots % 16] = torch.randn(37, 3, 2, 2, 64, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+
+    def tokens(r):
+        t = torch.tensor(list(m.requests[r].tables[0]))
+        p = torch.arange(m.requests[r].cursor)
+        return st[:, :, t[p // 16], :, p % 16].clone()
+
+    was = tokens("a")
+    m.fork("a", "b")
+    assert torch.equal(tokens("b"), was)
+    m.reserve("b", 5)
+    new = torch.from_numpy(m.slot_map(0, ["b"], [5])).long()
+    m.accept("b", 4)
+    st[:, :, new // 16, :, new % 16] = 9.0
+    assert torch.equal(tokens("a"), was) and torch.equal(tokens("b")[:37], was) and (tokens("b")[37:] == 9.0).all()
+    m.finish("a")
+    assert torch.equal(tokens("b")[:37], was)
+    m.check_invariants()
+
+
+class TreeDecoder:
+    """A small decoder out of the framework's kernels, a step of drafted trees: two layers of attention over a paged cache, with
+    rotary positions, and a head. Weights in 32 bits; ``dtype`` is that of the cache and the activations."""
+
+    V, H, NH, NKV, HD, LAYERS, PAGE = 97, 64, 4, 2, 64, 2, 16
+
+    def __init__(self, dtype, manager, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        self.dtype, self.m = dtype, manager
+        n = (self.NH + 2 * self.NKV) * self.HD
+
+        def w(*s, scale):
+            return (torch.randn(*s, generator=g) * scale).to(dtype).to(DEV)
+
+        self.embed = w(self.V, self.H, scale=1.0)
+        self.qkv = [w(n, self.H, scale=self.H ** -0.5) for _ in range(self.LAYERS)]
+        self.out = [w(self.H, self.NH * self.HD, scale=(self.NH * self.HD) ** -0.5) for _ in range(self.LAYERS)]
+        self.norm = torch.ones(self.H, device=DEV, dtype=dtype)
+        self.head = w(self.V, self.H, scale=2.0 * self.H ** -0.5)
+        self.inv_freq = (10000.0 ** (-torch.arange(0, self.HD, 2).float() / self.HD)).to(DEV)
+
+    def step(self, requests, tokens, parents):
+        """Logits [T, V] for each node of each request's tree, whose keys and values are then in the cache; and the batch."""
+        k = K()
+        q_lens = [len(t) for t in tokens]
+        flat = sum(tokens, [])
+        mask, depth = k.tree_plan(sum(parents, []), q_lens)
+        for r, n in zip(requests, q_lens):
+            self.m.reserve(r, n)
+        base = np.repeat([self.m.requests[r].cursor for r in requests], q_lens)
+        pos = torch.from_numpy(np.stack([base + depth] * 3).astype(np.int32)).to(DEV)
+        tok_seq = torch.from_numpy(np.repeat(np.arange(len(requests)), q_lens).astype(np.int32)).to(DEV)
+        cu = i32([0] + np.cumsum(q_lens).tolist()).to(DEV)
+        kv = [self.m.requests[r].cursor + n for r, n in zip(requests, q_lens)]
+        lens, bt = i32(kv).to(DEV), torch.from_numpy(self.m.block_table(0, requests)).to(DEV)
+        slots = torch.from_numpy(self.m.slot_map(0, requests, q_lens)).to(DEV)
+        zero = torch.zeros(len(requests), dtype=torch.int32, device=DEV)
+        cos, sin = k.rope_tables(pos, zero, tok_seq, cu, zero, torch.zeros(1, 2, dtype=torch.int32, device=DEV), self.inv_freq,
+                                 torch.zeros(self.HD // 2, dtype=torch.int32, device=DEV))
+        x, res = k.embed_lookup(self.embed, i32(flat).to(DEV), self.dtype), None
+        mask_d = torch.from_numpy(mask).to(DEV)
+        for l in range(self.LAYERS):
+            h, res = k.add_rmsnorm(x, res, self.norm, 1e-6, self.dtype)
+            y = k.linear(h, self.qkv[l], None, self.dtype)
+            st = self.m.groups[0].storage
+            k.rope_kv_write(y, cos, sin, st[l, 0], st[l, 1], slots, self.NH, self.NKV, self.HD, self.HD)
+            a = k.tree_attention(y, st[l, 0], st[l, 1], bt, cu, lens, mask_d, self.NH, self.NKV, self.HD, self.HD ** -0.5, None,
+                                 max(q_lens), max(kv), self.dtype)
+            x = k.linear(a, self.out[l], None, self.dtype)
+        h, _ = k.add_rmsnorm(x, res, self.norm, 1e-6, self.dtype)
+        return k.linear(h, self.head, None, F32), dict(cu_q=cu, seq_lens=lens, block_table=bt)
+
+
+def new_manager(dtype):
+    from omniserver_b200.cache import CacheManager
+    from omniserver_b200.models.decoder import EntryNeeds
+    from omniserver_b200.parts.base import KVCacheNeed
+    t = TreeDecoder
+    return CacheManager([EntryNeeds(KVCacheNeed(t.NKV, t.HD, None), [], None)] * t.LAYERS, [], t.PAGE, 60, 8, dtype, DEV, poison_freed=True)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_a_step_as_a_whole_emits_what_single_tokens_do(temperature):
+    """Prompts as chains, then steps of random trees: attention, verification, compaction, acceptance, forks in between. Greedy: the
+    tokens are those of decoding one by one. Sampled without draft probabilities, the root's children being all 97 words in an order
+    of chance, of which one is therefore accepted: the logits where the walk ended are those of a fresh request of the same tokens."""
+    rng = np.random.default_rng(4)
+    prompts = [rng.integers(0, 97, n).tolist() for n in (5, 23, 40)]
+
+    def chain(n):
+        return list(range(-1, n - 1))
+
+    # one by one
+    m1 = new_manager(F32)
+    d1 = TreeDecoder(F32, m1)
+    ids = [f"r{i}" for i in range(3)]
+    for r in ids:
+        m1.begin(r)
+    logits, _ = d1.step(ids, prompts, [chain(len(p)) for p in prompts])
+    ends = np.cumsum([len(p) for p in prompts]) - 1
+    for r, p in zip(ids, prompts):
+        m1.commit(r, len(p))
+    last = logits[torch.from_numpy(ends).to(DEV)].argmax(-1).tolist()
+    plain_tokens = [[t] for t in last]
+    for _ in range(24):
+        logits, _ = d1.step(ids, [[t[-1]] for t in plain_tokens], [[-1]] * 3)
+        for r in ids:
+            m1.commit(r, 1)
+        for t, w in zip(plain_tokens, logits.argmax(-1).tolist()):
+            t.append(w)
+    # by trees: the drafts are the right words at times
+    m2 = new_manager(F32)
+    d2 = TreeDecoder(F32, m2)
+    for r in ids:
+        m2.begin(r)
+    d2.step(ids, prompts, [chain(len(p)) for p in prompts])
+    for r, p in zip(ids, prompts):
+        m2.commit(r, len(p))
+    got = [[t] for t in last]
+    g = torch.Generator().manual_seed(5)
+    accepted = 0
+    for _ in range(12):
+        trees, parents = [], []
+        for i in range(3):
+            n = int(rng.integers(1, 14))
+            par = random_tree(n, rng)
+            depth = [0] * n
+            for j in range(1, n):
+                depth[j] = depth[par[j]] + 1
+            ahead = plain_tokens[i][len(got[i]):]
+            toks = [got[i][-1]] + [ahead[depth[j] - 1] if depth[j] <= len(ahead) and rng.random() < 0.7 else int(rng.integers(0, 97)) for j in range(1, n)]
+            if temperature > 0:   # every word below the root, then some nodes anywhere
+                par = [-1] + [0] * 97 + [int(rng.integers(0, 98)) for _ in range(n)]
+                toks = toks[:1] + rng.permutation(97).tolist() + rng.integers(0, 97, n).tolist()
+            trees.append(toks)
+            parents.append(par)
+        logits, batch = d2.step(ids, trees, parents)
+        T = sum(len(t) for t in trees)
+        u = (torch.randint(0, 1 << 24, (T,), generator=g).float() / (1 << 24)).to(DEV)
+        flat_t, flat_p = i32(sum(trees, [])).to(DEV), i32(sum(parents, [])).to(DEV)
+        new, path, count = K().verify_drafts(logits, flat_t, flat_p, batch["cu_q"], u, 128, 13, temperature=torch.full((3,), temperature, device=DEV))
+        want = plain.verify(logits.cpu(), flat_t.cpu(), flat_p.cpu(), batch["cu_q"].cpu(), u.cpu(), 13, torch.full((3,), temperature))
+        assert [list(x) for x in zip(new.tolist(), path.tolist(), count.tolist())] == [list(w) for w in want]
+        K().compact_cache(m2.groups[0].storage, batch["block_table"], batch["cu_q"], batch["seq_lens"], path, count)
+        if temperature > 0:
+            # a fresh request of the same tokens sees the same logits where the walk ended
+            t0 = 0
+            for i in range(3):
+                seq = prompts[i] + got[i][:-1] + [trees[i][j] for j in path[i, :int(count[i])].tolist()]
+                m2.begin("fresh")
+                ref, _ = d2.step(["fresh"], [seq], [chain(len(seq))])
+                m2.rollback("fresh")
+                m2.finish("fresh")
+                node = int(path[i, int(count[i]) - 1])
+                assert torch.allclose(logits[t0 + node], ref[-1], rtol=1e-3, atol=1e-3)
+                t0 += len(trees[i])
+        for i, r in enumerate(ids):
+            c = int(count[i])
+            accepted += c - 1
+            m2.accept(r, c)
+            got[i] += new[i, :c].tolist()
+            if temperature == 0.0:
+                assert got[i][:25] == plain_tokens[i][:len(got[i])][:25]
+        m2.check_invariants()
+        # a fork goes on from here like its parent would
+        m2.fork("r1", "child")
+        fl, _ = d2.step(["child"], [[got[1][-1]]], [[-1]])
+        pl, _ = d2.step(["r1"], [[got[1][-1]]], [[-1]])
+        assert torch.equal(fl, pl)
+        m2.rollback("r1")
+        m2.finish("child")
+        if temperature > 0 and min(len(x) for x in got) > 24:
+            break
+    assert accepted > 5
+    K().check_device_errors()
