@@ -35,8 +35,8 @@ constexpr int STAT_STAGES = 2;         // slices of a warp in shared memory: the
 constexpr int STAT_CTAS = 6;           // of the first kernel on an SM: 24 warps of 8 KB
 constexpr int PER_LANE = SLICE / 32;
 constexpr int MAX_CLUSTER = 8;
-constexpr float MIN_TEMP = 1e-30f;     // smaller ones are taken as this: log2(e) / T has to stay finite
-enum : int { ERR_TOKEN = 5 };
+constexpr float MIN_TEMP = 1e-30f, MAX_TEMP = 1e38f;   // others are taken as these: log2(e) / T is finite and has all its bits
+enum : int { ERR_TOKEN = 5, ERR_BOUNDS = 7 };
 
 struct SliceStat {
   double sum;    // of the weights against the slice's own maximum
@@ -47,7 +47,7 @@ struct SliceStat {
 // log2(e) / T, right to the last place: a division in 32 bits and its remainder (a division in 64 takes some 500 cycles)
 __device__ __forceinline__ float log2e_over(float t) {
   constexpr float HI = 1.44269502f, LO = (float)(1.4426950408889634074 - (double)HI);
-  t = fmaxf(t, MIN_TEMP);
+  t = fminf(fmaxf(t, MIN_TEMP), MAX_TEMP);
   const float q = HI / t;
   return fmaf(fmaf(-q, t, HI) + LO, q * 0.69314718f, q);
 }
@@ -57,8 +57,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// A slice whose maximum is infinite, or so large that its product with c is: the weights are then those of the differences.
-__device__ __forceinline__ bool odd_slice(float m, float c) { return !(fabsf(m * c) < INFINITY); }
+// A slice whose maximum is infinite, or so large that the rounding of m c is no small number any more (half a unit of 2^22 is 1/4; at
+// a temperature of 1e-8 it would be 128, and the weights out of range): the weights are then those of the differences l - m.
+__device__ __forceinline__ bool odd_slice(float m, float c) { return !(fabsf(m * c) < 4194304.0f); }
 // The weight of a word of an ordinary slice, mc = m * c; 0 for -inf and NaN (the maximum of a number and NaN is the number).
 __device__ __forceinline__ float weight(float l, float c, float mc) { return ex2(fmaxf(fmaf(l, c, -mc), -200.0f)); }
 __device__ __forceinline__ float weight_any(float l, float m, float c) {
@@ -66,12 +67,17 @@ __device__ __forceinline__ float weight_any(float l, float m, float c) {
   if (m == -INFINITY) return 0.0f;
   return l == m ? 1.0f : ex2(fmaxf((l - m) * c, -200.0f));
 }
-// A slice's factor against its row's maximum: exact to some 2^-22 like a weight, and then used in 64 bits.
+// A slice's factor against its row's maximum, from the numbers that the weights of both were taken against (m c rounded, or exactly m c
+// in an odd slice): exact to some 2^-22 like a weight, and then used in 64 bits.
 __device__ __forceinline__ double factor(float m, float m_row, float c) {
   if (m == -INFINITY) return 0.0;
   if (m == m_row) return 1.0;
-  if (!odd_slice(m, c) && !odd_slice(m_row, c)) return (double)ex2(fmaxf(m * c - m_row * c, -200.0f));
-  return m_row == INFINITY ? 0.0 : (double)ex2(fmaxf((m - m_row) * c, -200.0f));
+  if (m_row == INFINITY) return 0.0;
+  const float mc = m * c, rc = m_row * c;
+  float x;
+  if (!odd_slice(m, c)) x = odd_slice(m_row, c) ? fmaf(-m_row, c, mc) : __fsub_rn(mc, rc);
+  else x = odd_slice(m_row, c) ? (m - m_row) * c : fmaf(m, c, -rc);
+  return (double)ex2(fmaxf(x, -200.0f));
 }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -283,6 +289,7 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
   const int q0 = cu_q[s], q1 = cu_q[s + 1];
   const float tempf = temperature != nullptr ? temperature[s] : 0.0f;
   const int n = min(q1 - q0, max_nodes);
+  if (n < q1 - q0 && crank == 0 && tid == 0) atomicExch(err, ERR_BOUNDS);
   const int width = max_depth + 1;
   int* my_tokens = out_tokens + (size_t)s * width;
   int* my_path = out_path + (size_t)s * width;

@@ -193,7 +193,8 @@ class SpeculativeOps:
         softmax(logits / temperature) behind its parent less what the siblings rejected before it took: max(r - q, 0)
         renormalised, or without ``draft_probs`` (drafts that are certain of their token) the word itself. ``draft_probs`` [T, V]
         fp32: row i is the distribution that node i's children were drawn from; negative and NaN entries count as 0. NaN logits
-        count as -inf; where no logit of a row is above -inf nothing is accepted and the next token is 0.
+        count as -inf; where no logit of a row is above -inf nothing is accepted and the next token is 0. ``max_q_len``: at least the
+        most nodes of a request; what a larger one has beyond it is not looked at, and ``check_device_errors`` reports it.
 
         Out: ``path`` the accepted nodes from 0 on, ``tokens`` the new tokens (the accepted nodes' and the next one), both -1
         behind the first ``count``: that many nodes stay in the cache, and that many tokens are new. At most ``max_depth``

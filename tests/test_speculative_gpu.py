@@ -662,6 +662,50 @@ def test_copy_pages_refuses():
     assert torch.equal(cache, before)
 
 
+@pytest.mark.parametrize("dense", [False, True])
+def test_verify_reports_a_request_with_more_nodes_than_the_call_allowed(dense):
+    from omniserver_b200.ops import KernelError
+    args, q = drafts([4, 9], 300, seed=9, branch=1, dense=dense)
+    temp = torch.ones(2)
+    _, whole = verify_both(args, 9, 8, temp, q)
+    dev = {n: t.to(DEV) for n, t in args.items()}
+    got = K().verify_drafts(**dev, max_q_len=8, max_depth=8, temperature=temp.to(DEV), draft_probs=None if q is None else q.to(DEV))
+    with pytest.raises(KernelError, match="more nodes or keys"):
+        K().check_device_errors()
+    assert got[0][0].tolist() == whole[0][0] and got[1][0].tolist() == whole[0][1]
+    K().check_device_errors()
+
+
+@pytest.mark.parametrize("temp", [1e-38, 1e-12, 1e-8, 1e-7, 1e-6, 1e-5, 1e5, 1e30, math.inf])
+def test_verify_extreme_temperatures(temp):
+    """Logits with ties at the top. (The oracle takes 1e38 for infinity: behind that a difference of ordinary logits is nothing either way.)"""
+    args, _ = drafts([6, 5], 3001, seed=3)
+    args["logits"].clamp_(-12, 12)
+    got = K().verify_drafts(**{n: t.to(DEV) for n, t in args.items()}, max_q_len=6, max_depth=5, temperature=torch.full((2,), temp, device=DEV))
+    want = plain.verify(args["logits"], args["tokens"], args["parents"], args["cu_q"], args["uniform"], 5, torch.full((2,), min(temp, 1e38)))
+    assert [list(x) for x in zip(got[0].tolist(), got[1].tolist(), got[2].tolist())] == [list(w) for w in want]
+    K().check_device_errors()
+
+
+@pytest.mark.parametrize("dense", [False, True])
+@pytest.mark.parametrize("top", [3e6, 5e6])
+def test_verify_slices_of_very_different_size(top, dense):
+    """Logits a little apart around `top`, where m c rounds by halves, beside slices of small ones and of ones just below: with c = log2(e),
+    the maxima lie on both sides of 2^22."""
+    g = torch.Generator().manual_seed(6)
+    V = 4 * 1024
+    args, q = drafts([5, 4], V, seed=8, dense=dense)
+    x = torch.randn(9, V, generator=g)
+    x[:, :1024] = top + torch.randint(-3, 4, (9, 1024), generator=g) * 0.5
+    x[:, 2 * 1024:][:, :1024] = top * 0.9999995 + torch.randint(-3, 4, (9, 1024), generator=g) * 0.5
+    args["logits"] = x
+    for j in range(1, 9):
+        args["tokens"][j] = int(torch.randint(0, 1024, (1,), generator=g))
+    got, want = verify_both(args, 5, 4, torch.ones(2), q)
+    assert got == want
+    K().check_device_errors()
+
+
 # ------------------------------------------------------------------ streams, graphs, devices, and a step as a whole
 def device_step(step):
     d = {n: getattr(step, n).to(DEV) for n in ("qkv", "k", "v", "bt", "cu", "lens", "mask", "depth")}
@@ -986,4 +1030,44 @@ def test_a_step_as_a_whole_emits_what_single_tokens_do(temperature):
         if temperature > 0 and min(len(x) for x in got) > 24:
             break
     assert accepted > 5
+    K().check_device_errors()
+
+
+# ------------------------------------------------------------------ caches that 32-bit offsets do not reach
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tree_attention_in_a_cache_of_more_than_2_to_the_32_elements(dtype):
+    """The same pages, once in a small pool and once spread up to the end of one of 2^32 elements and more: the same bits."""
+    s = Step([9, 3], [200, 75], 4, 2, 128, 32, dtype, seed=4)
+    used = s.k.shape[0]
+    pages = (1 << 32) // (2 * 32 * 128) + 7
+    move = torch.arange(used, dtype=torch.long) * ((pages - 1) // (used - 1))
+    move[-1] = pages - 1
+    k = torch.empty(pages, 2, 32, 128, dtype=dtype, device=DEV)
+    v = torch.empty(pages, 2, 32, 128, dtype=dtype, device=DEV)
+    k[move.to(DEV)], v[move.to(DEV)] = s.k.to(DEV), s.v.to(DEV)
+    bt = torch.where(s.bt >= 0, move[s.bt.clamp(min=0).long()].to(torch.int32), -1)
+    want = s.got()
+    d = [t.to(DEV) for t in (s.qkv, bt, s.cu, s.lens, s.mask)]
+    got = K().tree_attention(d[0], k, v, *d[1:], 4, 2, 128, 128 ** -0.5, None, 9, 209, dtype)
+    assert torch.equal(got, want)
+    K().check_device_errors()
+
+
+def test_cache_operators_in_a_cache_of_more_than_2_to_the_32_bytes():
+    layers, nkv, page, hd = 3, 2, 16, 64
+    pages = (1 << 32) // (2 * layers * nkv * page * hd) + 5
+    cache = torch.empty(layers, 2, pages, nkv, page, hd, dtype=BF16, device=DEV)
+    ids = [pages - 1, 3, pages - 2]
+    rows = torch.randn(layers, 2, 3, nkv, page, hd, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+    at = torch.tensor(ids, device=DEV)
+    cache[:, :, at] = rows
+    K().copy_pages(cache, [pages - 1, 3], [pages - 4, 0])
+    assert torch.equal(cache[:, :, pages - 4], rows[:, :, 0]) and torch.equal(cache[:, :, 0], rows[:, :, 1])
+    dev = [i32(x).to(DEV) for x in ([ids], [0, 20], [45], [[0, 4, 18, -1]], [3])]
+    K().compact_cache(cache, *dev)
+    want = rows.clone()
+    for i, n in ((1, 4), (2, 18)):
+        a, b = 25 + n, 25 + i
+        want[:, :, b // page, :, b % page] = rows[:, :, a // page, :, a % page]
+    assert torch.equal(cache[:, :, at], want)
     K().check_device_errors()
