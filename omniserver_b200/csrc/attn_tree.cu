@@ -345,7 +345,9 @@ OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, 
                           int hd, int page_size, int num_pages, float scale, int window, int max_q_len, int max_kv_len,
                           float* scratch, int* err, cudaStream_t stream) {
   if (S <= 0 || max_q_len <= 0) return OSB_OK;
-  if (hd <= 0 || nkv <= 0 || nh % nkv != 0 || page_size <= 0 || (window > 0 && depth == nullptr)) return OSB_ERR_BAD_SHAPE;
+  if (hd <= 0 || nkv <= 0 || nh % nkv != 0 || page_size <= 0 || (window > 0 && depth == nullptr) ||
+      (max_q_len - 1) / 32 >= mask_words)
+    return OSB_ERR_BAD_SHAPE;
   if (hd > 256) return OSB_ERR_UNSUPPORTED;
   if (S > 65535 || nkv > 65535 || max_kv_len > MAX_KEYS) return OSB_ERR_TOO_LARGE;
   const long long need = osb_attn_tree_scratch(S, nh, nkv, hd, max_q_len, max_kv_len);

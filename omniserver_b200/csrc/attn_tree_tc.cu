@@ -516,6 +516,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     const uint32_t s_addr = tmem + ((uint32_t)(qd * 32) << 16), o_addr = s_addr + O_COL + (uint32_t)(half * (HD / 2));
     int i0 = 0, n_done = 0, u = 0;
     bool stop = false;
+    auto gave_up = [&] {
+      if (lane == 0) {
+        if (!*vabort) atomicExch(err, 113);
+        *vabort = 1;
+      }
+      __syncwarp();
+    };
     for (; !stop && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
       const int tok = r < seg.rows ? seg.r.q0 + seg.node0 + div_by(r, plan.inv_grp) : -1;   // this row's token, or none
       int lo_row = 0;
@@ -529,7 +536,12 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         if (masked && tok >= 0) sees = sees32(seg.r, plan, tok, lo_row, key0 + half * 32);
         if (!mbar_wait(&s_full[b], (uint32_t)(u >> 1) & 1u, vabort)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) {
+          // the other warp of these rows may still have got its scores: it must find this one at the barriers of every tile
+          gave_up();
+          if (pair_bar_or(qd, false)) pair_bar_or(qd, false);
+          continue;
+        }
         fence_after();
         const uint32_t sb = s_addr + (uint32_t)(b * TILE_N);
         uint32_t v[32];
@@ -635,7 +647,10 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
             fence_async_smem();
           }
         }
-        if (!ok) break;
+        if (!ok) {
+          gave_up();
+          continue;
+        }
         tmem_st_wait();
         fence_before();
         __syncwarp();
@@ -647,10 +662,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       if (walk.g >= walk.hi) pdl_trigger();        // the last stretch of this CTA
       stop = softmax_bar_or(!ok || *vabort != 0);
       if (stop) {
-        if (lane == 0) {
-          if (!*vabort) atomicExch(err, 113);
-          *vabort = 1;
-        }
+        gave_up();
         break;
       }
       const bool cut = !seg.whole, bad = found_bad[n_done & 1] != 0;
@@ -910,6 +922,7 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   Sizes z;
   if (num_pages <= 0 || !sizes_of(z, S, nh, nkv, hd, page_size, q_row_stride, scale, window, max_q_len, max_kv_len))
     return OSB_ERR_UNSUPPORTED;
+  if ((max_q_len - 1) / 32 >= mask_words) return OSB_ERR_BAD_SHAPE;
   if (((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15))
     return OSB_ERR_UNSUPPORTED;
   if ((window > 0 && depth == nullptr) || scratch == nullptr || ((uintptr_t)scratch & 15)) return OSB_ERR_BAD_SHAPE;

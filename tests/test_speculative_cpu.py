@@ -235,6 +235,29 @@ def test_tree_attention_entry_refuses(over, status):
     assert library.load().osb_attn_tree(*tree_args(**over)) == status
 
 
+@pytest.mark.parametrize("over", [
+    dict(hd=80), dict(hd=0), dict(nh=5), dict(nkv=0), dict(nh=129 * 2), dict(page=4), dict(page=24), dict(stride=516), dict(scale=0.0),
+    dict(scale=-1.0), dict(scale=float("nan")), dict(max_q=(1 << 24) + 1), dict(max_kv=(1 << 30) + 1), dict(max_kv=0), dict(window=-1),
+    dict(S=1 << 26, max_q=1024), dict(S=1 << 20, max_kv=1 << 20)])
+def test_tensor_core_tree_attention_does_not_take(over):
+    a = dict(S=1, nh=4, nkv=2, hd=64, page=16, stride=512, scale=1.0, window=0, max_q=4, max_kv=64)
+    a.update(over)
+    lib, scale = library.load(), ctypes.c_float(a["scale"])
+    lib.osb_attn_tree_tc_scratch.restype = ctypes.c_longlong
+    assert lib.osb_attn_tree_tc_scratch(a["S"], a["nh"], a["nkv"], a["hd"], a["page"], a["stride"], scale, a["window"], a["max_q"],
+                                        a["max_kv"]) == 0
+    assert lib.osb_attn_tree_tc(NULL, NULL, a["stride"], 4, NULL, NULL, NULL, 4, NULL, NULL, NULL, 1, NULL, a["S"], a["nh"], a["nkv"], a["hd"],
+                                a["page"], 4, scale, a["window"], a["max_q"], a["max_kv"], NULL, NULL, NULL) == UNSUPPORTED
+
+
+def test_tree_entries_refuse_too_few_mask_words():
+    lib = library.load()
+    args = list(tree_args(max_q=33))
+    assert lib.osb_attn_tree(*args) == BAD_SHAPE
+    assert lib.osb_attn_tree_tc(NULL, NULL, 512, 64, NULL, NULL, NULL, 4, NULL, NULL, NULL, 1, NULL, 1, 4, 2, 64, 16, 4, ctypes.c_float(1.0), 0, 33, 64, NULL, NULL,
+                                NULL) == BAD_SHAPE
+
+
 def test_scratch_of_the_32_bit_tree_attention_holds_every_smaller_request():
     """A request's rows x ranges never need more than what the largest request of its batch was given."""
     f = library.load().osb_attn_tree_scratch
