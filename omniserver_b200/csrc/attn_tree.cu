@@ -389,3 +389,5 @@ OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, 
     });
   });
 }
+OSB_PACKED(osb_attn_tree)
+OSB_PACKED(osb_attn_tree_scratch)

@@ -975,3 +975,5 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   if (hd == 64) return launch<64>(mq, mk, mv, (bf16*)out, part, (const bf16*)v_cache, p, z, scale_log2, stream);
   return launch<128>(mq, mk, mv, (bf16*)out, part, (const bf16*)v_cache, p, z, scale_log2, stream);
 }
+OSB_PACKED(osb_attn_tree_tc)
+OSB_PACKED(osb_attn_tree_tc_scratch)

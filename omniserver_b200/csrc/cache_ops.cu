@@ -169,3 +169,5 @@ OSB_API int osb_copy_pages(void* cache, long long page_bytes, int planes, int nu
     return osb_last_error();
   });
 }
+OSB_PACKED(osb_compact_cache)
+OSB_PACKED(osb_copy_pages)

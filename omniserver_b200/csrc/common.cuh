@@ -4,8 +4,10 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 #include <atomic>
+#include <type_traits>
 #include <utility>
 
 #define OSB_API extern "C" __attribute__((visibility("default")))
@@ -145,6 +147,29 @@ static inline int osb_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
                              Args&&... args) {
   return osb_launch_cluster(kernel, grid, block, smem, stream, 1, std::forward<Args>(args)...);
 }
+
+// An entry point a second time, with its arguments in an array of 64-bit words (pointers and integers as integers, numbers as doubles).
+// A caller in Python packs them in half a microsecond; 26 arguments one by one are converted in four.
+template <typename T> static inline T osb_word(const long long* w) {
+  if constexpr (std::is_pointer<T>::value) {
+    return reinterpret_cast<T>(static_cast<uintptr_t>(*w));
+  } else if constexpr (std::is_floating_point<T>::value) {
+    double d;
+    memcpy(&d, w, sizeof d);
+    return static_cast<T>(d);
+  } else {
+    return static_cast<T>(*w);
+  }
+}
+template <typename R, typename... A, size_t... I>
+static inline long long osb_call_packed(R (*f)(A...), const long long* words, std::index_sequence<I...>) {
+  return f(osb_word<A>(words + I)...);
+}
+template <typename R, typename... A> static inline long long osb_call_packed(R (*f)(A...), const long long* words) {
+  return osb_call_packed(f, words, std::index_sequence_for<A...>{});
+}
+#define OSB_PACKED(entry) \
+  OSB_API long long entry##_packed(const long long* words) { return osb_call_packed(entry, words); }
 
 // Dispatch over the two storage types: f(Tag<T>{}) is called with T = float or bf16.
 template <typename T> struct Tag { typedef T type; };

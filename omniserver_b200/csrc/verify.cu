@@ -711,3 +711,4 @@ OSB_API int osb_verify_drafts(int* out_tokens, int* out_path, int* out_count, vo
   }
   return rc ? rc : osb_last_error();
 }
+OSB_PACKED(osb_verify_drafts)

@@ -25,7 +25,7 @@ from .library import KernelLibraryError
 
 from ._common import _DEVICE_ERR, _STATUS, KernelError, _check, _cuda_contig, _dt, _p
 from .persistent import PersistentDecodeOps
-from .speculative import SpeculativeOps, declare
+from .speculative import Entries, SpeculativeOps
 
 
 class CudaKernels(PersistentDecodeOps, SpeculativeOps):
@@ -44,7 +44,7 @@ class CudaKernels(PersistentDecodeOps, SpeculativeOps):
 
     def __init__(self) -> None:
         self.lib = library.load()
-        declare(self.lib)
+        self._entries = Entries(self.lib)
         # the library GEMM (used for medium row counts) must accumulate in fp32, also across its K splits
         torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
         self._err: Dict[int, torch.Tensor] = {}

@@ -14,6 +14,7 @@ The reference has none of these (it decodes one token per request and step, omni
 from __future__ import annotations
 
 import ctypes
+import struct
 from operator import index
 from typing import List, Optional, Sequence, Tuple
 
@@ -24,26 +25,31 @@ from ._common import KernelError, _check, _cuda_contig, _dt
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
-_PTR, _INT, _FLOAT, _LONG = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
-_SIGNATURES = {
-    "osb_attn_tree_scratch": [_INT, _INT, _INT, _INT, _INT, _INT],
-    "osb_attn_tree": [_PTR, _INT, _PTR, _INT, _INT, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT,
-                      _INT, _INT, _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR],
-    "osb_attn_tree_tc_scratch": [_INT, _INT, _INT, _INT, _INT, _INT, _FLOAT, _INT, _INT, _INT],
-    "osb_attn_tree_tc": [_PTR, _PTR, _INT, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _INT, _INT, _INT, _INT, _INT,
-                         _FLOAT, _INT, _INT, _INT, _PTR, _PTR, _PTR],
-    "osb_verify_drafts": [_PTR] * 11 + [_INT] * 5 + [_PTR, _PTR],
-    "osb_compact_cache": [_PTR, _INT, _INT, _INT, _INT, _INT, _INT, _PTR, _INT, _PTR, _PTR, _PTR, _INT, _PTR, _INT, _PTR, _PTR],
-    "osb_copy_pages": [_PTR, _LONG, _INT, _INT, _PTR, _PTR, _INT, _PTR],
+# The arguments of the entry points: Q an address (0: none), q an integer, d a number.
+_ENTRIES = {
+    "attn_tree_scratch": "qqqqqq",
+    "attn_tree": "QqQqqQQqQqQQQqQqqqqqqdqqqQQQ",
+    "attn_tree_tc_scratch": "qqqqqqdqqq",
+    "attn_tree_tc": "QQqqQQQqQQQqQqqqqqqdqqqQQQ",
+    "verify_drafts": "QQQQQQQQQQQqqqqqQQ",
+    "compact_cache": "QqqqqqqQqQQQqQqQQ",
+    "copy_pages": "QqqqQQqQ",
 }
 
 
-def declare(lib: ctypes.CDLL) -> None:
-    """The argument types of this file's entry points, so that plain integers can be handed over as addresses: these calls are made
-    where a step's launches take a few microseconds, and an object per address costs about as much."""
-    for name, types in _SIGNATURES.items():
-        getattr(lib, name).argtypes = types
-    lib.osb_attn_tree_scratch.restype = lib.osb_attn_tree_tc_scratch.restype = _LONG
+class Entries:
+    """This file's entry points of the library, ``osb_attn_tree`` as ``attn_tree(...)`` and so on, with every call's arguments packed
+    into one array: these calls are made where a step's launches take a few microseconds, and converting 26 arguments one by
+    one takes four."""
+
+    def __init__(self, lib: ctypes.CDLL):
+        for name, args in _ENTRIES.items():
+            setattr(self, name, self._entry(getattr(lib, f"osb_{name}_packed"), struct.Struct("=" + args).pack))
+
+    @staticmethod
+    def _entry(fn, pack):
+        fn.argtypes, fn.restype = [ctypes.c_char_p], ctypes.c_longlong
+        return lambda *args: fn(pack(*args))
 
 
 def _on_device(ref: torch.Tensor) -> int:
@@ -55,10 +61,11 @@ def _on_device(ref: torch.Tensor) -> int:
     return dev
 
 
-def _operands(dev: int, dtype: Optional[torch.dtype], **tensors: torch.Tensor) -> None:
-    """Contiguous tensors of this type on this device."""
-    for name, t in tensors.items():
+def _operands(dev: int, dtype: Optional[torch.dtype], names: str, *tensors: torch.Tensor) -> None:
+    """Contiguous tensors of this type on this device; ``names``: theirs, for the message."""
+    for t in tensors:
         if t.get_device() != dev or (dtype is not None and t.dtype is not dtype) or not t.is_contiguous():
+            name = names.split()[next(i for i, x in enumerate(tensors) if x is t)]
             _cuda_contig(name, t, dtype)
             raise KernelError(f"{name} must be on cuda:{dev}")
 
@@ -125,9 +132,9 @@ class SpeculativeOps:
         ``exact=True`` and shapes the tensor-core kernel does not take run in 32 bits throughout.
         """
         dev = _on_device(qkv)
-        _operands(dev, None, qkv=qkv, k_cache=k_cache, v_cache=v_cache)
-        _operands(dev, _I32, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, tree_mask=tree_mask)
-        win = int(window) if window else 0
+        _operands(dev, None, "qkv k_cache v_cache", qkv, k_cache, v_cache)
+        _operands(dev, _I32, "block_table cu_q seq_lens tree_mask", block_table, cu_q, seq_lens, tree_mask)
+        win = min(int(window), 1 << 30) if window else 0      # (no request has more keys)
         _check(win >= 0, "tree_attention: a window is positive")
         _check(qkv.dim() == 2 and seq_lens.dim() == 1 and block_table.dim() == 2 and tree_mask.dim() == 2 and k_cache.dim() == 4,
                "tree_attention: qkv [T,*], seq_lens [S], block_table [S,*], tree_mask [T,W], caches [pages, nkv, page_size, hd]")
@@ -144,39 +151,40 @@ class SpeculativeOps:
         _check(cu_q.shape == (S + 1,), "tree_attention: cu_q [S+1]")
         _check(rows == T and 32 * words >= max_q_len, "tree_attention: tree_mask [T, W] with 32 W >= max_q_len")
         _check(hd <= 256, "tree_attention: head sizes up to 256")
+        _check(max_kv_len <= 1 << 30, "tree_attention: up to 2^30 keys per request")
         if depth is not None:
-            _operands(dev, _I32, depth=depth)
+            _operands(dev, _I32, "depth", depth)
             _check(depth.shape == (T,), "tree_attention: depth [T]")
         else:
             _check(win == 0, "tree_attention: a window needs the nodes' depth")
         if out is None:
-            out = torch.empty((T, nh * hd), dtype=out_dtype, device=qkv.device)
+            out = qkv.new_empty((T, nh * hd)) if out_dtype is qkv.dtype else qkv.new_empty((T, nh * hd), dtype=out_dtype)
         else:
-            _operands(dev, out_dtype, out=out)
+            _operands(dev, out_dtype, "out", out)
             _check(out.shape == (T, nh * hd), "tree_attention: out [T, nh*hd]")
         if S == 0 or T == 0 or max_q_len <= 0 or max_kv_len <= 0 or pages == 0:
             return out
         qp, kp, vp, op = qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-        dp = depth.data_ptr() if depth is not None else None
+        dp = depth.data_ptr() if depth is not None else 0
         err = self.err_flag(qkv.device).data_ptr()
         need = 0
         if (not exact and qkv.dtype is _BF16 and k_cache.dtype is _BF16 and out_dtype is _BF16 and (qp | kp | vp | op) % 16 == 0):
-            need = self.lib.osb_attn_tree_tc_scratch(S, nh, nkv, hd, page_size, width, scale, win, max_q_len, max_kv_len)
+            need = self._entries.attn_tree_tc_scratch(S, nh, nkv, hd, page_size, width, scale, win, max_q_len, max_kv_len)
         if need > 0:
-            scratch = torch.empty(need, dtype=torch.uint8, device=qkv.device)
-            rc = self.lib.osb_attn_tree_tc(
+            scratch = qkv.new_empty(need, dtype=torch.uint8)
+            rc = self._entries.attn_tree_tc(
                 op, qp, width, T, kp, vp, block_table.data_ptr(), bt_width, cu_q.data_ptr(), seq_lens.data_ptr(),
                 tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len, max_kv_len,
                 scratch.data_ptr(), err, self._raw_stream(dev))
             self._ok(rc, "attn_tree_tc")
             self.launches += 1 if max_kv_len > 64 else 0
         else:
-            need = self.lib.osb_attn_tree_scratch(S, nh, nkv, hd, max_q_len, max_kv_len)
-            scratch = torch.empty(need, dtype=_F32, device=qkv.device) if need > 0 else None
-            rc = self.lib.osb_attn_tree(
+            need = self._entries.attn_tree_scratch(S, nh, nkv, hd, max_q_len, max_kv_len)
+            scratch = qkv.new_empty(need, dtype=_F32) if need > 0 else None
+            rc = self._entries.attn_tree(
                 op, _dt(out), qp, _dt(qkv), width, kp, vp, _dt(k_cache), block_table.data_ptr(), bt_width, cu_q.data_ptr(),
                 seq_lens.data_ptr(), tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len,
-                max_kv_len, scratch.data_ptr() if need > 0 else None, err, self._raw_stream(dev))
+                max_kv_len, scratch.data_ptr() if need > 0 else 0, err, self._raw_stream(dev))
             self._ok(rc, "attn_tree")
             self.launches += 1 if need > 0 else 0
         return out
@@ -202,8 +210,8 @@ class SpeculativeOps:
         reported by ``check_device_errors`` where a request brings it as a draft.
         """
         dev = _on_device(logits)
-        _operands(dev, _F32, logits=logits, uniform=uniform)
-        _operands(dev, _I32, tokens=tokens, parents=parents, cu_q=cu_q)
+        _operands(dev, _F32, "logits uniform", logits, uniform)
+        _operands(dev, _I32, "tokens parents cu_q", tokens, parents, cu_q)
         _check(logits.dim() == 2 and cu_q.dim() == 1 and cu_q.shape[0] >= 1, "verify_drafts: logits [T,V], cu_q [S+1]")
         T, V = logits.shape
         S = cu_q.shape[0] - 1
@@ -212,27 +220,23 @@ class SpeculativeOps:
                "verify_drafts: tokens, parents and uniform [T]")
         _check(0 <= max_q_len <= self.MAX_TREE_NODES, "verify_drafts: up to 1024 nodes per request")
         _check(max_depth >= 0, "verify_drafts: max_depth must not be negative")
-        tp = qp = None
+        tp = qp = 0
         if temperature is not None:
-            _operands(dev, _F32, temperature=temperature)
+            _operands(dev, _F32, "temperature", temperature)
             _check(temperature.shape == (S,), "verify_drafts: temperature [S]")
             tp = temperature.data_ptr()
         if draft_probs is not None:
-            _operands(dev, _F32, draft_probs=draft_probs)
+            _operands(dev, _F32, "draft_probs", draft_probs)
             _check(draft_probs.shape == (T, V), "verify_drafts: draft_probs [T,V]")
             qp = draft_probs.data_ptr()
-        # the three results, and behind them, on a 16-byte boundary, 16 bytes per slice of a row for the kernels
-        w = max_depth + 1
-        n = S * w
-        head = (2 * n + S + 3) & ~3
-        buf = torch.empty(head + 4 * T * -(-V // self.VERIFY_SLICE), dtype=_I32, device=logits.device)
-        new, path, count = buf[:n].view(S, w), buf[n:2 * n].view(S, w), buf[2 * n:2 * n + S]
+        shape = (S, max_depth + 1)
+        new, path, count = tokens.new_empty(shape), tokens.new_empty(shape), tokens.new_empty(S)
         if S == 0:
             return new, path, count
-        at = buf.data_ptr()
-        rc = self.lib.osb_verify_drafts(at, at + 4 * n, at + 8 * n, at + 4 * head, logits.data_ptr(), tokens.data_ptr(),
-                                        parents.data_ptr(), cu_q.data_ptr(), uniform.data_ptr(), tp, qp, S, T, V, max_q_len,
-                                        max_depth, self.err_flag(logits.device).data_ptr(), self._raw_stream(dev))
+        stats = tokens.new_empty(4 * T * -(-V // self.VERIFY_SLICE))      # 16 bytes per slice of a row
+        rc = self._entries.verify_drafts(new.data_ptr(), path.data_ptr(), count.data_ptr(), stats.data_ptr(), logits.data_ptr(),
+                                         tokens.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), uniform.data_ptr(), tp, qp, S, T, V,
+                                         max_q_len, max_depth, self.err_flag(logits.device).data_ptr(), self._raw_stream(dev))
         self._ok(rc, "verify_drafts")
         self.launches += 1 if T > 0 else 0
         return new, path, count
@@ -242,7 +246,7 @@ class SpeculativeOps:
     def _storage(cache: torch.Tensor) -> Tuple[int, Tuple[int, ...]]:
         """(device index, shape) of a page group's storage."""
         dev = _on_device(cache)
-        _operands(dev, None, cache=cache)
+        _operands(dev, None, "cache", cache)
         _check(cache.dim() == 6 and cache.shape[1] == 2, "cache must be [layers, 2, pages, nkv, page_size, hd]")
         _dt(cache)
         return dev, cache.shape
@@ -256,7 +260,7 @@ class SpeculativeOps:
         it moves nothing of its request, and a token in a page outside the pool stays; both are reported by
         ``check_device_errors``."""
         dev, (L, _, P, nkv, ps, hd) = self._storage(cache)
-        _operands(dev, _I32, block_table=block_table, cu_q=cu_q, seq_lens=seq_lens, path=path, count=count)
+        _operands(dev, _I32, "block_table cu_q seq_lens path count", block_table, cu_q, seq_lens, path, count)
         S = seq_lens.shape[0]
         _check(seq_lens.dim() == 1 and cu_q.shape == (S + 1,) and count.shape == (S,),
                "compact_cache: seq_lens, count [S], cu_q [S+1]")
@@ -264,9 +268,10 @@ class SpeculativeOps:
         _check(path.dim() == 2 and path.shape[0] == S, "compact_cache: path [S,*]")
         if S == 0 or cache.numel() == 0:
             return
-        rc = self.lib.osb_compact_cache(cache.data_ptr(), cache.element_size(), 2 * L, P, nkv, ps, hd, block_table.data_ptr(),
-                                        block_table.shape[1], cu_q.data_ptr(), seq_lens.data_ptr(), path.data_ptr(),
-                                        path.shape[1], count.data_ptr(), S, self.err_flag(cache.device).data_ptr(), self._raw_stream(dev))
+        rc = self._entries.compact_cache(cache.data_ptr(), cache.element_size(), 2 * L, P, nkv, ps, hd, block_table.data_ptr(),
+                                         block_table.shape[1], cu_q.data_ptr(), seq_lens.data_ptr(), path.data_ptr(),
+                                         path.shape[1], count.data_ptr(), S, self.err_flag(cache.device).data_ptr(),
+                                         self._raw_stream(dev))
         self._ok(rc, "compact_cache")
 
     def copy_pages(self, cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
@@ -285,6 +290,6 @@ class SpeculativeOps:
             return
         pages = (ctypes.c_int * (2 * n))(*a, *b)
         at = ctypes.addressof(pages)
-        rc = self.lib.osb_copy_pages(cache.data_ptr(), nkv * ps * hd * cache.element_size(), 2 * L, P, at, at + 4 * n, n,
-                                     self._raw_stream(dev))
+        rc = self._entries.copy_pages(cache.data_ptr(), nkv * ps * hd * cache.element_size(), 2 * L, P, at, at + 4 * n, n,
+                                      self._raw_stream(dev))
         self._ok(rc, "copy_pages")
