@@ -39,6 +39,7 @@ constexpr int BLOCK_M = 128, TILE_N = 64;
 constexpr int NUM_THREADS = 384, CTAS_PER_SM = 2;
 constexpr int Q_ATOM = BLOCK_M * 128, KV_ATOM = TILE_N * 128;   // rows of 128 bytes
 constexpr int MIN_PIECE = 2;                         // key tiles of a CTA at least
+constexpr int OTHER_REGS = 64, SOFTMAX_REGS = 88;    // of a thread
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
 
@@ -368,7 +369,10 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   walk.m = plan.abreast > 1 ? (int)blockIdx.x - group * plan.abreast : 0;
   if (plan.abreast > 1 && walk.m >= start_r.m_tiles) walk.hi = walk.g;     // the request has fewer row tiles than it might
   Seg seg;
-
+  // The softmax warps take registers over from the others: 128 x 64 + 256 x 88 = the 384 x 80 of the launch. (Without, and with 48 and
+  // 96, something is kept in local memory, whose first use alone costs a microsecond: one request 13.8 us instead of 12.7.)
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------------ TMA producers: warp 0 keys, warp 2 values
     // Lane b looks up the page of box b; one thread issues all copies of a tile one after the other (a copy per lane would be
@@ -379,18 +383,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     int last[2] = {-1, -1}; // numbers of the tiles that this warp put into the ring last
     for (; !*vabort && walk.next(plan, seg); i0 += 2 * seg.n_tiles) {
       const int p_last = seg.r.kv_len - 1;
-      // a page outside the pool reads as zeros; it is reported unless every row's window has passed it (then it was given back)
-      auto page_of = [&](int t) -> int {
+      auto page_of = [&](int t) -> int {      // of this lane's box of tile t
         const int key = (seg.tile_begin + t) * TILE_N + lane * box_rows;
-        if (t >= seg.n_tiles || lane >= n_boxes || key > p_last) return -1;
-        const int page = seg.bt[key >> log2ps];
-        if (page >= 0 && page < plan.num_pages) return page;
-        if (plan.window <= 0 || key + box_rows > seg.r.base - plan.window + 1) atomicExch(err, ERR_PAGE);
-        return -1;
+        return t >= seg.n_tiles || lane >= n_boxes || key > p_last ? -1 : seg.bt[key >> log2ps];
       };
       int page = page_of(0), next_page = page_of(1);
       for (int t = 0; t < seg.n_tiles && !*vabort; ++t) {
-        const int after_next = page_of(t + 2);  // in flight while these tiles' copies are issued
+        const int after_next = page_of(t + 2);  // in flight while these tiles' copies are issued (nothing looks at it yet)
         const int i = i0 + (keys ? (t == 0 ? 0 : 2 * t - 1) : (t + 1 < seg.n_tiles ? 2 * t + 2 : 2 * t + 1)), st = i % STAGES;
         const int key0 = (seg.tile_begin + t) * TILE_N;
         // whole boxes (pages) up to the request's last key; a box that starts beyond it is skipped
@@ -402,6 +401,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
           } else {
             mbar_expect_tx(&full[st], (uint32_t)(boxes * NA * box_rows * 128));
           }
+        }
+        // a page outside the pool reads as zeros; it is reported unless every row's window has passed it (then it was given back)
+        if ((unsigned)page >= (unsigned)plan.num_pages) {
+          page = -1;
+          const int key = key0 + lane * box_rows;
+          if (lane < n_boxes && key <= p_last && (plan.window <= 0 || key + box_rows > seg.r.base - plan.window + 1))
+            atomicExch(err, ERR_PAGE);
         }
         __syncwarp();
         if (*vabort) break;
@@ -430,13 +436,29 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ issuer of S = Q K^T
+    // ------------------------------------------------------------------ loads Q, issues S = Q K^T
     // (the whole warp goes through the loops, one thread issues: the descriptors then stay in uniform registers)
     constexpr uint32_t idesc_s = make_idesc(BLOCK_M, TILE_N, 0, 0);
     const uint64_t q_desc = desc_kmajor(q_smem), k_desc = desc_kmajor(ring);
-    bool ok = true;
-    int i0 = 0, n_done = 0, u = 0;
+    bool ok = true, staged = false;      // staged: the stretch before stages its output where Q lies
+    int i0 = 0, n_done = 0, u = 0, q_issued = 0;
     for (; ok && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
+      // Q goes where the stretch before had its own: until its last scores are complete, or, if it stages its output there, until
+      // that has left (epi_done, followed phase by phase, at most one behind)
+      if (n_done > 1) ok = mbar_wait(&epi_done, (uint32_t)n_done & 1u, vabort);
+      if (n_done > 0 && staged) ok = ok && mbar_wait(&epi_done, (uint32_t)(n_done - 1) & 1u, vabort);
+      if (n_done > 0 && !staged) ok = ok && mbar_wait(&s_full[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u, vabort);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(&q_full, (uint32_t)(NA * plan.nodes_per_tile * plan.grp * 128));
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+          tma_load_3d(q_smem + a * Q_ATOM, &map_q, &q_full, a * 64, seg.kvh * plan.grp, seg.r.q0 + seg.node0);
+      }
+      __syncwarp();
+      q_issued = n_done + 1;
+      staged = seg.whole;
       ok = mbar_wait(&q_full, (uint32_t)n_done & 1u, vabort);
       for (int t = 0; t < seg.n_tiles; ++t, ++u) {
         const int i = i0 + (t == 0 ? 0 : 2 * t - 1), st = i % STAGES, b = u & 1;
@@ -458,29 +480,21 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         __syncwarp();
       }
     }
-    if (!ok && lane == 0) {
-      if (!*vabort) atomicExch(err, 112);
-      *vabort = 1;
+    if (!ok) {
+      if (lane == 0) {
+        if (!*vabort) atomicExch(err, 112);
+        *vabort = 1;
+      }
+      for (uint32_t w = 0; q_issued > 0 && w < WAIT_LIMIT && !mbar_try_wait(&q_full, (uint32_t)(q_issued - 1) & 1u); ++w) {
+      }
     }
   } else if (warp == 3) {
-    // ------------------------------------------------------------------ loads Q, issues O += P V
+    // ------------------------------------------------------------------ issuer of O += P V
     constexpr uint32_t idesc_o = make_idesc(BLOCK_M, HD, 0, 1);  // B = V: N (head dim) contiguous
     const uint64_t v_desc = desc_mnmajor(ring, KV_ATOM);
     bool ok = true;
-    int i0 = 0, n_done = 0, q_issued = 0, u = 0;
-    for (; ok && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
-      // Q goes where the stretch before staged its output: wait until that has left
-      if (n_done > 0 && !mbar_wait(&epi_done, (uint32_t)(n_done - 1) & 1u, vabort)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (elect_one()) {
-        mbar_expect_tx(&q_full, (uint32_t)(NA * plan.nodes_per_tile * plan.grp * 128));
-#pragma unroll
-        for (int a = 0; a < NA; ++a)
-          tma_load_3d(q_smem + a * Q_ATOM, &map_q, &q_full, a * 64, seg.kvh * plan.grp, seg.r.q0 + seg.node0);
-      }
-      __syncwarp();
-      q_issued = n_done + 1;
+    int i0 = 0, u = 0;
+    for (; ok && walk.next(plan, seg); i0 += 2 * seg.n_tiles) {
       for (int t = 0; t < seg.n_tiles; ++t, ++u) {
         const int i = i0 + (t + 1 < seg.n_tiles ? 2 * t + 2 : 2 * t + 1), st = i % STAGES, b = u & 1;
         ok = mbar_wait(&p_full[b], (uint32_t)(u >> 1) & 1u, vabort) && mbar_wait(&full[st], (uint32_t)(i / STAGES) & 1u, vabort);
@@ -491,7 +505,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < TILE_N / 16; ++ks)
-            umma_bf16_ts(tmem + O_COL, tmem + (uint32_t)(b * TILE_N + ks * 8), bd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o,
+            umma_bf16_ts(tmem + O_COL, tmem + (uint32_t)(b * TILE_N + (ks >> 1) * 32 + (ks & 1) * 8), bd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o,
                          (t > 0 || ks > 0) ? 1u : 0u);
           umma_commit(&pv_done[b]);
           umma_commit(&empty[st]);
@@ -499,15 +513,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         __syncwarp();
       }
     }
-    if (!ok) {
-      if (lane == 0) {
-        if (!*vabort) atomicExch(err, 112);
-        *vabort = 1;
-      }
-      for (uint32_t w = 0; q_issued > 0 && w < WAIT_LIMIT && !mbar_try_wait(&q_full, (uint32_t)(q_issued - 1) & 1u); ++w) {
-      }
+    if (!ok && lane == 0) {
+      if (!*vabort) atomicExch(err, 112);
+      *vabort = 1;
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     // ------------------------------------------------------------------ softmax and epilogue: eight warps
     const int qd = warp & 3;             // TMEM lane quarter of this warp
     const int half = (warp - 4) >> 2;    // of a tile's keys, and of the output's columns
@@ -534,7 +546,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         const bool masked = tile_masked(seg.r, plan, key0);
         unsigned sees = 0u;
         if (masked && tok >= 0) sees = sees32(seg.r, plan, tok, lo_row, key0 + half * 32);
-        if (!mbar_wait(&s_full[b], (uint32_t)(u >> 1) & 1u, vabort)) ok = false;
+        if (ok && !mbar_wait(&s_full[b], (uint32_t)(u >> 1) & 1u, vabort)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
           // the other warp of these rows may still have got its scores: it must find this one at the barriers of every tile
@@ -543,9 +555,8 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
           continue;
         }
         fence_after();
-        const uint32_t sb = s_addr + (uint32_t)(b * TILE_N);
-        uint32_t v[32];
-        tmem_ld32(sb + (uint32_t)(half * 32), v);
+        uint32_t v[32];                            // the scores of this half's keys
+        tmem_ld32(s_addr + (uint32_t)(b * TILE_N + half * 32), v);
         tmem_ld_wait();
         if (masked) {
 #pragma unroll
@@ -560,7 +571,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
             mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;  // the scale is positive
         // the exponent offset in use moves only when the maximum has grown enough (or at the first keys); what lies in rows
-        // that are none moves nothing. (The barrier also says that both warps have read their scores: P goes over them.)
+        // that are none moves nothing
         bool grow = tok >= 0 && (mx > m_run + RESCALE_THRESHOLD || (m_run == -INFINITY && mx > -INFINITY));
         if (pair_bar_or(qd, grow)) {
           row_max[b][half][r] = mx;
@@ -604,7 +615,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
           __nv_bfloat162 w = __floats2bfloat162_rn(p0, p1);
           pk[j >> 1] = *reinterpret_cast<uint32_t*>(&w);
         }
-        tmem_st16(sb + (uint32_t)(half * 16), pk);
+        tmem_st16(s_addr + (uint32_t)(b * TILE_N + half * 32), pk);
         float s0, s1;
         unpack2(add2(sum_a, sum_b), s0, s1);
         l_run += s0 + s1;
