@@ -243,7 +243,7 @@ struct Layout {
 //  full / empty: a place of the ring has its tile / the products that read it have completed. Tiles pass through the ring in the
 //    order K0, K1, V0, K2, V1, .. of a stretch, numbered on across stretches: tile i is in place i % STAGES.
 //  s_full: Q K^T of key tile u is in S. p_full: its P is there (and V may be read). pv_done: P V complete, so S / P may be overwritten,
-//    and, of a stretch's last tile, O read. q_full / epi_done: a stretch's Q has landed / its output has left O and Q's place.
+//    and, of a stretch's last tile, O read. q_full / staged_out: a stretch's Q has landed / a staged output has left Q's place.
 template <int HD>
 __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -255,10 +255,10 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* q_smem = base;
   unsigned char* ring = base + Q_BYTES;               // STAGES tiles of keys or values
-  __shared__ uint64_t q_full, epi_done, full[STAGES], empty[STAGES], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint64_t q_full, staged_out, full[STAGES], empty[STAGES], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int found_bad[2];            // by the parity of the CTA's stretches: values that are not finite were taken out of a V tile
+  __shared__ int found_bad[3];            // by the number of the CTA's stretch modulo 3: values that are not finite were taken out of a V tile
   __shared__ int scan[NUM_THREADS / 32];
   __shared__ int start_s, start_p;        // the request in which this CTA's piece begins, where its units begin
   __shared__ Req start_r;
@@ -274,10 +274,10 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   if (lane == 0 && warp < 3) prefetch_tensormap(warp == 0 ? &map_k : warp == 1 ? &map_q : &map_v);
   if (tid == 0) {
     abort_flag = 0;
-    found_bad[0] = found_bad[1] = 0;
+    found_bad[0] = found_bad[1] = found_bad[2] = 0;
     start_s = 0;
     mbar_init(&q_full, 1);
-    mbar_init(&epi_done, 8);
+    mbar_init(&staged_out, 8);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -441,13 +441,12 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     constexpr uint32_t idesc_s = make_idesc(BLOCK_M, TILE_N, 0, 0);
     const uint64_t q_desc = desc_kmajor(q_smem), k_desc = desc_kmajor(ring);
     bool ok = true, staged = false;      // staged: the stretch before stages its output where Q lies
-    int i0 = 0, n_done = 0, u = 0, q_issued = 0;
+    int i0 = 0, n_done = 0, u = 0, q_issued = 0, n_staged = 0;
     for (; ok && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
       // Q goes where the stretch before had its own: until its last scores are complete, or, if it stages its output there, until
-      // that has left (epi_done, followed phase by phase, at most one behind)
-      if (n_done > 1) ok = mbar_wait(&epi_done, (uint32_t)n_done & 1u, vabort);
-      if (n_done > 0 && staged) ok = ok && mbar_wait(&epi_done, (uint32_t)(n_done - 1) & 1u, vabort);
-      if (n_done > 0 && !staged) ok = ok && mbar_wait(&s_full[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u, vabort);
+      // that has left. (staged_out has a phase for each stretch of that kind, and this warp sees every one of them.)
+      if (staged) ok = mbar_wait(&staged_out, (uint32_t)(n_staged - 1) & 1u, vabort);
+      else if (n_done > 0) ok = mbar_wait(&s_full[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u, vabort);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (elect_one()) {
@@ -459,6 +458,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       __syncwarp();
       q_issued = n_done + 1;
       staged = seg.whole;
+      n_staged += staged ? 1 : 0;
       ok = mbar_wait(&q_full, (uint32_t)n_done & 1u, vabort);
       for (int t = 0; t < seg.n_tiles; ++t, ++u) {
         const int i = i0 + (t == 0 ? 0 : 2 * t - 1), st = i % STAGES, b = u & 1;
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     const int r = qd * 32 + lane;        // query row of this thread
     const int ts = tid - 128;
     const uint32_t s_addr = tmem + ((uint32_t)(qd * 32) << 16), o_addr = s_addr + O_COL + (uint32_t)(half * (HD / 2));
-    int i0 = 0, n_done = 0, u = 0;
+    int i0 = 0, u = 0, bad_slot = 0;
     bool stop = false;
     auto gave_up = [&] {
       if (lane == 0) {
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       }
       __syncwarp();
     };
-    for (; !stop && walk.next(plan, seg); i0 += 2 * seg.n_tiles, ++n_done) {
+    for (; !stop && walk.next(plan, seg); i0 += 2 * seg.n_tiles, bad_slot = bad_slot == 2 ? 0 : bad_slot + 1) {
       const int tok = r < seg.rows ? seg.r.q0 + seg.node0 + div_by(r, plan.inv_grp) : -1;   // this row's token, or none
       int lo_row = 0;
       if (plan.window > 0 && tok >= 0) lo_row = seg.r.base + min(max(plan.depth[tok], 0), seg.r.n - 1) - plan.window + 1;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
                 any |= not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
               }
               if (any) {
-                found_bad[n_done & 1] = 1;
+                found_bad[bad_slot] = 1;
 #pragma unroll 1
                 for (int c = 0; c < 2 * NA; ++c) {
                   uint4 w = *piece_at(c0 + c);
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         gave_up();
         break;
       }
-      const bool cut = !seg.whole, bad = found_bad[n_done & 1] != 0;
+      const bool cut = !seg.whole, bad = found_bad[bad_slot] != 0;
       const int slot = 2 * (int)blockIdx.x + (seg.began ? 0 : 1);
       float4* po = part_o + (size_t)slot * (HD / 4) * BLOCK_M + r;
       // One range of keys: O / l as bf16 through the shared memory that held Q (every product that read it has completed), so that
@@ -746,11 +746,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         }
       }
       if (!seg.began && ts == 0) plan.cuts[seg.unit] = Cut{(int)blockIdx.x, seg.pieces};     // for the second kernel
-      if (ts == 0) found_bad[(n_done + 1) & 1] = 0;   // last read between the barriers of the stretch before
+      // the slot of the stretch before, and of the one after the next: everyone read it before this stretch's barrier, and no one
+      // writes it before the next one's
+      if (ts == 0) found_bad[bad_slot == 0 ? 2 : bad_slot - 1] = 0;
       // what this warp read of O (tensor memory) and of the staged rows is in its registers or on its way out
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&epi_done);
+      if (!cut && lane == 0) mbar_arrive(&staged_out);
     }
   }
   fence_before();

@@ -1071,3 +1071,33 @@ def test_cache_operators_in_a_cache_of_more_than_2_to_the_32_bytes():
         want[:, :, b // page, :, b % page] = rows[:, :, a // page, :, a % page]
     assert torch.equal(cache[:, :, at], want)
     K().check_device_errors()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_tree_attention_over_and_over(hd):
+    """Batches whose requests are cut at many places, or fit in whole, in many calls: the same bits every time, no wait given up."""
+    rng = np.random.default_rng(8)
+    for bases in (rng.integers(1500, 2200, 64).tolist(), rng.integers(0, 300, 200).tolist(), [20000, 5, 700, 64, 3000]):
+        call = device_step(Step([int(x) for x in rng.integers(1, 9, len(bases))], bases, 28, 4, hd, 64, BF16, seed=8))[1]
+        want = call()
+        for _ in range(60):
+            outs = [call() for _ in range(5)]
+            assert all(torch.equal(o, want) for o in outs)
+    K().check_device_errors()
+
+
+def test_tree_attention_values_that_are_not_finite_in_neighbouring_stretches():
+    """Infinities in places that some rows see and others do not, in every request of a batch cut at many places: they reach the rows that
+    see them, in every one, and no others."""
+    step = Step([9] * 40, [100 + 37 * i for i in range(40)], 12, 2, 128, 32, BF16, seed=2)
+    for s in range(40):
+        at = step.bases[s] + 4                        # node 4: seen by itself and its descendants
+        step.v[int(step.bt[s, at // 32]), :, at % 32, :] = math.inf
+    got = step.got()
+    cu = step.cu.tolist()
+    words = step.mask[:, 0].tolist()
+    for s in range(40):
+        for t in range(cu[s], cu[s + 1]):
+            sees = (words[t] >> 4) & 1
+            assert bool((got[t] == math.inf).all()) if sees else bool(got[t].isfinite().all()), (s, t)
+    K().check_device_errors()
