@@ -38,7 +38,10 @@ using namespace attn_tree;
 constexpr int BLOCK_M = 128, TILE_N = 64;
 constexpr int NUM_THREADS = 384, CTAS_PER_SM = 2;
 constexpr int Q_ATOM = BLOCK_M * 128, KV_ATOM = TILE_N * 128;   // rows of 128 bytes
-constexpr int MIN_PIECE = 2;                         // key tiles of a CTA at least
+// Key tiles that a CTA takes beyond an even piece to have a unit whole, where there are no more units than CTAs: cutting costs the second
+// kernel and the way through scratch. Whole or cut, us: 3 requests of 87 keys and 4 kv heads (2 tiles) 8.7, 12.7; 8 of 320 and 2 heads
+// (5 tiles) 11.7, 13.9; with 10 instead of 6, 22 of 740 and 2 heads (12 tiles) 19.4, 14.0.
+constexpr int WHOLE_EXTRA = 6;
 constexpr int OTHER_REGS = 64, SOFTMAX_REGS = 88;    // of a thread
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in log2 units
@@ -59,6 +62,7 @@ struct Plan {
   Cut* cuts;           // scratch, by unit: (request x kv heads + head) x row tiles + tile
   int bt_stride, mask_words, S, nh, nkv, grp, log2ps, num_pages, window, max_q_len, kv_cap;
   int nodes_per_tile, m_tiles, ctas;
+  int whole_tiles;                  // key tiles of a unit at most, if there are no more units than CTAs (if there are: a huge number)
   int abreast;                      // row tiles that neighbouring CTAs take at the same time (1: row tiles are units like others)
   unsigned inv_nodes, inv_grp;      // 2^32 / nodes_per_tile and / grp, rounded up
 };
@@ -293,7 +297,10 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   // until here nothing was read that the kernel before this one in the stream may still be writing (lengths, q, the pages)
   pdl_wait();
 
-  // ---- this CTA's piece of the line of tiles
+  // ---- this CTA's piece of the line of tiles, or its unit
+  const int own = (int)blockIdx.x;
+  Req own_r = {};
+  if (plan.whole_tiles < MAX_KEYS) own_r = req_of(plan, min(own / (plan.nkv * plan.m_tiles), plan.S - 1));
   Req mine = {};                                // of request `tid`
   int my_tiles = 0;
   long long all = 0;
@@ -330,7 +337,8 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   // (row tiles abreast: a group of CTAs has one piece)
   const int groups = plan.abreast > 1 ? (int)gridDim.x / plan.abreast : (int)gridDim.x;
   const int group = plan.abreast > 1 ? (int)blockIdx.x / plan.abreast : (int)blockIdx.x;
-  const int piece = max(MIN_PIECE, (total + groups - 1) / groups);
+  const int piece = max(1, (total + groups - 1) / groups);
+  const bool whole = plan.whole_tiles <= piece + WHOLE_EXTRA;
   const int g0 = (int)min((long long)total, (long long)group * piece), g1 = group < groups ? min(total, g0 + piece) : g0;
   if (plan.S <= NUM_THREADS) {
     if (my_tiles > 0 && g0 >= first && g0 < first + my_tiles) {
@@ -367,6 +375,15 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   walk.r = start_r;
   walk.piece = piece;
   walk.m = plan.abreast > 1 ? (int)blockIdx.x - group * plan.abreast : 0;
+  if (whole) {
+    // this CTA's unit, or none
+    walk.s = own / (plan.nkv * plan.m_tiles);
+    walk.r = own_r;
+    const int unit = own - walk.s * plan.nkv * plan.m_tiles, kvh = unit / plan.m_tiles, m = unit - kvh * plan.m_tiles;
+    walk.p_s = 0;
+    walk.g = (kvh * own_r.m_tiles + m) * own_r.tiles;
+    walk.hi = own < plan.S * plan.nkv * plan.m_tiles && m < own_r.m_tiles ? walk.g + own_r.tiles : walk.g;
+  }
   if (plan.abreast > 1 && walk.m >= start_r.m_tiles) walk.hi = walk.g;     // the request has fewer row tiles than it might
   Seg seg;
   // The softmax warps take registers over from the others: 128 x 64 + 256 x 88 = the 384 x 80 of the launch. (Without, and with 48 and
@@ -745,7 +762,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
               *reinterpret_cast<const uint4*>(q_smem + row * (HD * 2) + ((c ^ (row & (CPR - 1))) << 4));
         }
       }
-      if (!seg.began && ts == 0) plan.cuts[seg.unit] = Cut{(int)blockIdx.x, seg.pieces};     // for the second kernel
+      if (plan.cuts != nullptr && !seg.began && ts == 0) plan.cuts[seg.unit] = Cut{(int)blockIdx.x, seg.pieces};     // for the second kernel
       // the slot of the stretch before, and of the one after the next: everyone read it before this stretch's barrier, and no one
       // writes it before the next one's
       if (ts == 0) found_bad[bad_slot == 0 ? 2 : bad_slot - 1] = 0;
@@ -861,7 +878,8 @@ int most_tiles(int max_q_len, int max_kv_len, int window) {
 }
 
 struct Sizes {
-  int grp, nodes, m_tiles, row_blocks, tiles, ctas, abreast;
+  int grp, nodes, m_tiles, row_blocks, tiles, ctas, abreast, whole_tiles;
+  bool cuts;                             // whether a unit may be cut: then there is a second kernel
   long long cut_bytes, part_floats;      // the scratch: the cuts, then the pieces
 };
 // 0 if the kernel does not take these shapes
@@ -882,8 +900,10 @@ bool sizes_of(Sizes& z, int S, int nh, int nkv, int hd, int page_size, int q_row
   const int most = CTAS_PER_SM * sms;
   z.ctas = line < most ? (int)line : most;
   z.abreast = S == 1 && z.m_tiles > 1 && z.m_tiles <= z.ctas ? z.m_tiles : 1;
-  z.cut_bytes = ((long long)S * nkv * z.m_tiles * (long long)sizeof(Cut) + 15) / 16 * 16;
-  z.part_floats = z.tiles > 1 ? (long long)2 * z.ctas * BLOCK_M * (hd + 2) : 0;
+  z.whole_tiles = z.abreast == 1 && (long long)S * nkv * z.m_tiles <= z.ctas ? z.tiles : MAX_KEYS;
+  z.cuts = z.tiles > 1 && z.whole_tiles > 1 + WHOLE_EXTRA;
+  z.cut_bytes = z.cuts ? ((long long)S * nkv * z.m_tiles * (long long)sizeof(Cut) + 15) / 16 * 16 : 0;
+  z.part_floats = z.cuts ? (long long)2 * z.ctas * BLOCK_M * (hd + 2) : 0;
   return true;
 }
 
@@ -896,7 +916,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   float2* ml = (float2*)(part + (long long)2 * z.ctas * BLOCK_M * HD);
   rc = osb_launch(attn_tree_tc_kernel<HD>, dim3((unsigned)z.ctas), dim3(NUM_THREADS), Layout<HD>::SMEM, stream, mq, mk, mv, out, po, ml,
                   v_cache, plan, scale_log2);
-  if (rc == 0 && z.part_floats > 0) {
+  if (rc == 0 && z.cuts) {
     const int units = plan.S * plan.nkv * plan.m_tiles;
     // warps for so many dims each and so many sharing the pieces of a row: as many as make about one wave. Both kernels with each
     // of the four, in this order, us: one request of 2,048 keys on 2 kv heads 13.7, 14.7, 15.7, 20.3; 8 ragged ones of up to 4,096
@@ -916,12 +936,12 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
 }
 }  // namespace
 
-// Bytes of scratch that osb_attn_tree_tc needs for these arguments, 0 if it does not take them.
+// Bytes of scratch that osb_attn_tree_tc needs for these arguments: 0 if it does not take them, 1 if it takes them and needs none.
 OSB_API long long osb_attn_tree_tc_scratch(int S, int nh, int nkv, int hd, int page_size, int q_row_stride, float scale, int window,
                                            int max_q_len, int max_kv_len) {
   Sizes z;
   if (!sizes_of(z, S, nh, nkv, hd, page_size, q_row_stride, scale, window, max_q_len, max_kv_len)) return 0;
-  return z.cut_bytes + z.part_floats * 4;
+  return z.cuts ? z.cut_bytes + z.part_floats * 4 : 1;
 }
 
 // As osb_attn_tree for bf16 operands; scratch: osb_attn_tree_tc_scratch bytes for the same arguments, on a 16-byte boundary. Shapes
@@ -938,7 +958,7 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   if ((max_q_len - 1) / 32 >= mask_words) return OSB_ERR_BAD_SHAPE;
   if (((uintptr_t)q & 15) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15))
     return OSB_ERR_UNSUPPORTED;
-  if ((window > 0 && depth == nullptr) || scratch == nullptr || ((uintptr_t)scratch & 15)) return OSB_ERR_BAD_SHAPE;
+  if ((window > 0 && depth == nullptr) || (z.cuts && (scratch == nullptr || ((uintptr_t)scratch & 15)))) return OSB_ERR_BAD_SHAPE;
   Plan p = {};
   p.block_table = block_table;
   p.cu_q = cu_q;
@@ -946,7 +966,7 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   p.mask = mask;
   p.depth = depth;
   p.err = err;
-  p.cuts = (Cut*)scratch;
+  p.cuts = z.cuts ? (Cut*)scratch : nullptr;
   p.bt_stride = bt_stride;
   p.mask_words = mask_words;
   p.S = S;
@@ -963,6 +983,7 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   p.m_tiles = z.m_tiles;
   p.ctas = z.ctas;
   p.abreast = z.abreast;
+  p.whole_tiles = z.whole_tiles;
   p.inv_nodes = z.nodes == 1 ? 0u : (unsigned)((0x100000000ull + z.nodes - 1) / z.nodes);
   p.inv_grp = z.grp == 1 ? 0u : (unsigned)((0x100000000ull + z.grp - 1) / z.grp);
   CUtensorMap mq, mk, mv;

@@ -171,13 +171,13 @@ class SpeculativeOps:
         if (not exact and qkv.dtype is _BF16 and k_cache.dtype is _BF16 and out_dtype is _BF16 and (qp | kp | vp | op) % 16 == 0):
             need = self._entries.attn_tree_tc_scratch(S, nh, nkv, hd, page_size, width, scale, win, max_q_len, max_kv_len)
         if need > 0:
-            scratch = qkv.new_empty(need, dtype=torch.uint8)
+            scratch = qkv.new_empty(need, dtype=torch.uint8) if need > 1 else None
             rc = self._entries.attn_tree_tc(
                 op, qp, width, T, kp, vp, block_table.data_ptr(), bt_width, cu_q.data_ptr(), seq_lens.data_ptr(),
                 tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len, max_kv_len,
-                scratch.data_ptr(), err, self._raw_stream(dev))
+                0 if scratch is None else scratch.data_ptr(), err, self._raw_stream(dev))
             self._ok(rc, "attn_tree_tc")
-            self.launches += 1 if max_kv_len > 64 else 0
+            self.launches += 1 if need > 1 else 0      # the second kernel, which joins what was cut
         else:
             need = self._entries.attn_tree_scratch(S, nh, nkv, hd, max_q_len, max_kv_len)
             scratch = qkv.new_empty(need, dtype=_F32) if need > 0 else None
