@@ -188,7 +188,8 @@ class CacheManager:
 
     def fork(self, parent_id: str, child_id: str) -> RequestCache:
         """A new request with the parent's tokens in its cache, between two steps: it shares the parent's full pages, gets a copy
-        of the partly filled one, and a slot with a copy of the parent's state. All or nothing."""
+        of the partly filled one, and a slot with a copy of the parent's state. All or nothing. (A newest token that only the device
+        knows is the runner's, not the cache's: the child's first step brings its own.)"""
         parent = self.requests[parent_id]
         if parent.reserved:
             raise ValueError(f"request {parent_id!r} cannot be forked while a step of it runs")

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(
     int q_row_stride, const KVT* __restrict__ k_cache, const KVT* __restrict__ v_cache, const int* __restrict__ block_table,
     int bt_stride, const int* __restrict__ cu_q, const int* __restrict__ seq_lens, const unsigned* __restrict__ mask,
     int mask_words, const int* __restrict__ depth, int nh, int nkv, int hd, int page_size, int num_pages, float scale,
-    int window, int max_ranges, int cap_rows, int max_q_len, int kv_cap, int* __restrict__ err) {
+    int window, int max_ranges, int cap_rows, int max_q_len, int kv_cap, int T, int* __restrict__ err) {
   constexpr int LD = HDP + 4;
   constexpr int ND = HDP / 64;       // 4-dim pieces of an output row per thread
   extern __shared__ __align__(16) float sm[];
@@ -80,6 +80,10 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(
   const int split = blockIdx.x % max_ranges, tile = blockIdx.x / max_ranges;
   const int kvh = blockIdx.y, s = blockIdx.z;
   const int q0 = cu_q[s], n = cu_q[s + 1] - q0;
+  if (q0 < 0 || n < 0 || q0 + n > T) {        // tokens that are not there
+    if (tile == 0 && split == 0 && threadIdx.x == 0) atomicExch(err, ERR_BOUNDS);
+    return;
+  }
   const int grp = nh / nkv, rows = min(n, max_q_len) * grp, r0 = tile * RT;
   if (r0 >= rows) return;
   const int kv_all = seq_lens[s], kv_len = min(kv_all, kv_cap);
@@ -266,10 +270,11 @@ template <typename OT>
 __global__ void __launch_bounds__(128) attn_tree_join_kernel(OT* __restrict__ out, const float* __restrict__ part_o,
                                                              const float* __restrict__ part_ml, const int* __restrict__ cu_q,
                                                              const int* __restrict__ seq_lens, int nh, int nkv, int hd,
-                                                             int max_q_len, int kv_cap, int cap_rows) {
+                                                             int max_q_len, int kv_cap, int cap_rows, int T) {
   constexpr int HELD = MAX_CTAS / 32;       // ranges whose weights a lane has: k, k + 32, ..
   pdl_wait();
-  const int s = blockIdx.z, kvh = blockIdx.y, q0 = cu_q[s], n = min(cu_q[s + 1] - q0, max_q_len);
+  const int s = blockIdx.z, kvh = blockIdx.y, q0 = cu_q[s], q1 = cu_q[s + 1], n = min(q1 - q0, max_q_len);
+  if (q0 < 0 || q1 > T) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = nh / nkv, rows = n * grp, r = blockIdx.x * 4 + warp;
   if (r >= rows) return;
@@ -339,12 +344,12 @@ OSB_API long long osb_attn_tree_scratch(int S, int nh, int nkv, int hd, int max_
 // (needed with a window; below the request's number of nodes), scratch: osb_attn_tree_scratch floats for the same arguments.
 // max_q_len / max_kv_len: at least the largest of the batch; a request beyond them is reported in *err, and what lies beyond is
 // not computed.
-OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, int q_row_stride, const void* k_cache,
+OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, int q_row_stride, int T, const void* k_cache,
                           const void* v_cache, int cache_dtype, const int* block_table, int bt_stride, const int* cu_q,
                           const int* seq_lens, const unsigned* mask, int mask_words, const int* depth, int S, int nh, int nkv,
                           int hd, int page_size, int num_pages, float scale, int window, int max_q_len, int max_kv_len,
                           float* scratch, int* err, cudaStream_t stream) {
-  if (S <= 0 || max_q_len <= 0) return OSB_OK;
+  if (S <= 0 || T <= 0 || max_q_len <= 0) return OSB_OK;
   if (hd <= 0 || nkv <= 0 || nh % nkv != 0 || page_size <= 0 || (window > 0 && depth == nullptr) ||
       (max_q_len - 1) / 32 >= mask_words)
     return OSB_ERR_BAD_SHAPE;
@@ -375,7 +380,7 @@ OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, 
           return osb_launch(k, dim3((unsigned)(tiles * ranges), (unsigned)nkv, (unsigned)S), dim3(NT), smem, stream, (OT*)out,
                             part_o, (float*)part_ml, (const QT*)q, q_row_stride, (const KVT*)k_cache, (const KVT*)v_cache, block_table,
                             bt_stride, cu_q, seq_lens, mask, mask_words, depth, nh, nkv, hd, page_size, num_pages, scale,
-                            window, ranges, cap_rows, max_q_len, kv_cap, err);
+                            window, ranges, cap_rows, max_q_len, kv_cap, T, err);
         };
         int rc = hdp == 64    ? go(attn_tree_kernel<QT, KVT, OT, 64>, osb_allow_smem<attn_tree_kernel<QT, KVT, OT, 64>>(smem))
                  : hdp == 128 ? go(attn_tree_kernel<QT, KVT, OT, 128>, osb_allow_smem<attn_tree_kernel<QT, KVT, OT, 128>>(smem))
@@ -383,7 +388,7 @@ OSB_API int osb_attn_tree(void* out, int out_dtype, const void* q, int q_dtype, 
         if (rc == 0 && need > 0)
           rc = osb_launch(attn_tree_join_kernel<OT>, dim3((unsigned)((max_rows + 3) / 4), (unsigned)nkv, (unsigned)S), dim3(128), 0,
                           stream, (OT*)out, (const float*)part_o, (const float*)part_ml, cu_q, seq_lens, nh, nkv, hd, max_q_len,
-                          kv_cap, cap_rows);
+                          kv_cap, cap_rows, T);
         return rc ? rc : osb_last_error();
       });
     });

@@ -60,7 +60,7 @@ struct Plan {
   const int* depth;
   int* err;
   Cut* cuts;           // scratch, by unit: (request x kv heads + head) x row tiles + tile
-  int bt_stride, mask_words, S, nh, nkv, grp, log2ps, num_pages, window, max_q_len, kv_cap;
+  int T, bt_stride, mask_words, S, nh, nkv, grp, log2ps, num_pages, window, max_q_len, kv_cap;
   int nodes_per_tile, m_tiles, ctas;
   int whole_tiles;                  // key tiles of a unit at most, if there are no more units than CTAs (if there are: a huge number)
   int abreast;                      // row tiles that neighbouring CTAs take at the same time (1: row tiles are units like others)
@@ -85,7 +85,7 @@ __device__ __forceinline__ Req req_of(const Plan& p, int s) {
   Req r;
   r.q0 = p.cu_q[s];
   const int q1 = p.cu_q[s + 1], kv_all = p.seq_lens[s];
-  r.n = q1 - r.q0;
+  r.n = r.q0 >= 0 && q1 <= p.T ? q1 - r.q0 : -1;       // (tokens that are not there: reported, and nothing is done)
   r.kv_len = min(kv_all, p.kv_cap);
   r.base = kv_all - r.n;
   const int lo = p.window > 0 && r.base - p.window + 1 > 0 ? min(r.base - p.window + 1, r.kv_len - 1) : 0;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       my_tiles = t;
     }
     all += t;
-    if (blockIdx.x == 0 && r.n > 0 && (r.kv_len < r.base + r.n || r.n > plan.max_q_len || r.base < 0)) atomicExch(err, ERR_BOUNDS);
+    if (blockIdx.x == 0 && r.n != 0 && (r.n < 0 || r.kv_len < r.base + r.n || r.n > plan.max_q_len || r.base < 0)) atomicExch(err, ERR_BOUNDS);
   }
   auto block_scan = [&](int v, int& total) -> int {      // exclusive
     int inc = v;
@@ -969,6 +969,7 @@ OSB_API int osb_attn_tree_tc(void* out, const void* q, int q_row_stride, int T, 
   p.cuts = z.cuts ? (Cut*)scratch : nullptr;
   p.bt_stride = bt_stride;
   p.mask_words = mask_words;
+  p.T = T;
   p.S = S;
   p.nh = nh;
   p.nkv = nkv;

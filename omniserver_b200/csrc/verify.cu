@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
     int* __restrict__ out_tokens, int* __restrict__ out_path, int* __restrict__ out_count,
     const SliceStat* __restrict__ stats, const float* __restrict__ logits, const int* __restrict__ tokens,
     const int* __restrict__ parents, const int* __restrict__ cu_q, const float* __restrict__ uniform,
-    const float* __restrict__ temperature, const float* __restrict__ draft_probs, int V, int n_slices, int max_nodes,
+    const float* __restrict__ temperature, const float* __restrict__ draft_probs, int T, int V, int n_slices, int max_nodes,
     int max_depth, int* __restrict__ err) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   WalkSmem& sh = *reinterpret_cast<WalkSmem*>(smem_raw);
@@ -288,8 +288,8 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
   pdl_wait();
   const int q0 = cu_q[s], q1 = cu_q[s + 1];
   const float tempf = temperature != nullptr ? temperature[s] : 0.0f;
-  const int n = min(q1 - q0, max_nodes);
-  if (n < q1 - q0 && crank == 0 && tid == 0) atomicExch(err, ERR_BOUNDS);
+  const int n = q0 >= 0 && q1 <= T ? min(q1 - q0, max_nodes) : -1;     // (tokens that are not there: none)
+  if ((n < 0 || n != q1 - q0) && crank == 0 && tid == 0) atomicExch(err, ERR_BOUNDS);
   const int width = max_depth + 1;
   int* my_tokens = out_tokens + (size_t)s * width;
   int* my_path = out_path + (size_t)s * width;
@@ -699,7 +699,7 @@ OSB_API int osb_verify_drafts(int* out_tokens, int* out_path, int* out_count, vo
     if (ready) return ready;
     return osb_launch_cluster(k, dim3((unsigned)(S * csize)), dim3(WALK_THREADS), smem, stream, csize, out_tokens, out_path,
                               out_count, (const SliceStat*)stats, logits, tokens, parents, cu_q, uniform, temperature,
-                              draft_probs, V, n_slices, max_nodes, max_depth, err);
+                              draft_probs, T, V, n_slices, max_nodes, max_depth, err);
   };
   if (draft_probs != nullptr && temperature != nullptr) {
     // a row of draft probabilities is summed by a cluster: of as many CTAs as let every request have its own at once, one per SM

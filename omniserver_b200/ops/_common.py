@@ -28,7 +28,7 @@ _DEVICE_ERR = {
     4: "a page index outside the page pool in attention",
     5: "a drafted token outside the vocabulary reached the verification",
     6: "a path that does not ascend within its tree reached the cache compaction",
-    7: "a request has more nodes or keys than the call (tree attention, verification) allowed for",
+    7: "a request has more nodes or keys than the call (tree attention, verification) allowed for, or tokens outside its rows",
     101: "tcgen05 GEMM: the TMA producer waited too long for a free stage",
     102: "tcgen05 GEMM: the MMA issuer waited too long for operands",
     103: "tcgen05 GEMM: the epilogue waited too long for the accumulator",

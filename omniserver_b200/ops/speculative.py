@@ -28,7 +28,7 @@ _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 # The arguments of the entry points: Q an address (0: none), q an integer, d a number.
 _ENTRIES = {
     "attn_tree_scratch": "qqqqqq",
-    "attn_tree": "QqQqqQQqQqQQQqQqqqqqqdqqqQQQ",
+    "attn_tree": "QqQqqqQQqQqQQQqQqqqqqqdqqqQQQ",
     "attn_tree_tc_scratch": "qqqqqqdqqq",
     "attn_tree_tc": "QQqqQQQqQQQqQqqqqqqdqqqQQQ",
     "verify_drafts": "QQQQQQQQQQQqqqqqQQ",
@@ -126,8 +126,9 @@ class SpeculativeOps:
         not count). With a ``window`` it sees the last ``window`` places up to its own, a node's place being base +
         ``depth`` [T] int32. A node that sees nothing gets zeros. What hidden places hold does not matter.
 
-        ``max_q_len`` / ``max_kv_len``: at least the most nodes and keys of a request; a larger one, and a page outside the pool
-        among the visible ones, is reported by ``check_device_errors``, and that request's rows are then not defined.
+        ``max_q_len`` / ``max_kv_len``: at least the most nodes and keys of a request; a larger one, tokens outside qkv, and a
+        page outside the pool among the visible ones, are reported by ``check_device_errors``, and that request's rows are
+        then not defined.
         Rows of ``out`` [T, nh*hd] (made here if not given) that belong to no request are not written. float32 operands,
         ``exact=True`` and shapes the tensor-core kernel does not take run in 32 bits throughout.
         """
@@ -182,7 +183,7 @@ class SpeculativeOps:
             need = self._entries.attn_tree_scratch(S, nh, nkv, hd, max_q_len, max_kv_len)
             scratch = qkv.new_empty(need, dtype=_F32) if need > 0 else None
             rc = self._entries.attn_tree(
-                op, _dt(out), qp, _dt(qkv), width, kp, vp, _dt(k_cache), block_table.data_ptr(), bt_width, cu_q.data_ptr(),
+                op, _dt(out), qp, _dt(qkv), width, T, kp, vp, _dt(k_cache), block_table.data_ptr(), bt_width, cu_q.data_ptr(),
                 seq_lens.data_ptr(), tree_mask.data_ptr(), words, dp, S, nh, nkv, hd, page_size, pages, scale, win, max_q_len,
                 max_kv_len, scratch.data_ptr() if need > 0 else 0, err, self._raw_stream(dev))
             self._ok(rc, "attn_tree")
@@ -202,7 +203,8 @@ class SpeculativeOps:
         renormalised, or without ``draft_probs`` (drafts that are certain of their token) the word itself. ``draft_probs`` [T, V]
         fp32: row i is the distribution that node i's children were drawn from; negative and NaN entries count as 0. NaN logits
         count as -inf; where no logit of a row is above -inf nothing is accepted and the next token is 0. ``max_q_len``: at least the
-        most nodes of a request; what a larger one has beyond it is not looked at, and ``check_device_errors`` reports it.
+        most nodes of a request; what a larger one has beyond it is not looked at, nor a request whose tokens are outside
+        ``logits`` (count 0), and ``check_device_errors`` reports them.
 
         Out: ``path`` the accepted nodes from 0 on, ``tokens`` the new tokens (the accepted nodes' and the next one), both -1
         behind the first ``count``: that many nodes stay in the cache, and that many tokens are new. At most ``max_depth``

@@ -223,7 +223,7 @@ def tree_args(**over):
     a = dict(S=1, nh=4, nkv=2, hd=64, page=16, pages=4, window=0, max_q=4, max_kv=64, depth=NULL, part=NULL, dtypes=(0, 0, 0))
     a.update(over)
     o, q, c = a["dtypes"]
-    return (NULL, o, NULL, q, 512, NULL, NULL, c, NULL, 4, NULL, NULL, NULL, 1, a["depth"], a["S"], a["nh"], a["nkv"], a["hd"],
+    return (NULL, o, NULL, q, 512, 64, NULL, NULL, c, NULL, 4, NULL, NULL, NULL, 1, a["depth"], a["S"], a["nh"], a["nkv"], a["hd"],
             a["page"], a["pages"], ctypes.c_float(1.0), a["window"], a["max_q"], a["max_kv"], a["part"], NULL, NULL)
 
 

@@ -1101,3 +1101,37 @@ def test_tree_attention_values_that_are_not_finite_in_neighbouring_stretches():
             sees = (words[t] >> 4) & 1
             assert bool((got[t] == math.inf).all()) if sees else bool(got[t].isfinite().all()), (s, t)
     K().check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cu", [[0, 5, 15], [-1, 5, 14], [0, 16, 14], [0, 5, 2]])
+def test_tree_attention_reports_tokens_that_are_not_there(dtype, cu):
+    """Offsets outside the rows of qkv, or falling: reported; rows outside are not written, and what is right is computed."""
+    from omniserver_b200.ops import KernelError
+    s = Step([5, 9], [30, 140], 4, 2, 64, 16, dtype, seed=2)
+    d = [t.to(DEV) for t in (s.qkv, s.k, s.v, s.bt, i32(cu), s.lens, s.mask)]
+    buf = torch.full((20, 256), 7.0, dtype=dtype, device=DEV)
+    K().tree_attention(*d, 4, 2, 64, 0.125, None, 9, 149, dtype, out=buf[3:17])
+    with pytest.raises(KernelError, match="tokens outside"):
+        K().check_device_errors()
+    assert (buf[:3] == 7.0).all() and (buf[17:] == 7.0).all()
+    if cu[:2] == [0, 5]:
+        assert torch.equal(buf[3:8], s.got(scale=0.125)[:5]) or dtype == BF16
+
+
+@pytest.mark.parametrize("dense", [False, True])
+def test_verify_reports_tokens_that_are_not_there(dense):
+    from omniserver_b200.ops import KernelError
+    args, q = drafts([4, 9], 300, seed=9, branch=1, dense=dense)
+    temp = torch.ones(2)
+    want = verify_both(args, 9, 8, temp, q)[1]
+    for cu in ([0, 4, 14], [-2, 4, 13], [0, 4, 2]):
+        dev = {n: t.to(DEV) for n, t in args.items()}
+        dev["cu_q"] = i32(cu).to(DEV)
+        new, path, count = K().verify_drafts(**dev, max_q_len=9, max_depth=8, temperature=temp.to(DEV), draft_probs=None if q is None else q.to(DEV))
+        with pytest.raises(KernelError, match="tokens outside"):
+            K().check_device_errors()
+        bad = 0 if cu[0] < 0 else 1
+        assert int(count[bad]) == 0 and (new[bad] == -1).all() and (path[bad] == -1).all()
+        if cu == [0, 4, 14]:
+            assert new[0].tolist() == want[0][0] and path[0].tolist() == want[0][1]
