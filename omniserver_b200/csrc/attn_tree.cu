@@ -10,8 +10,8 @@
 // are register tiles (4 rows x 2 keys, 4 rows x HD / 16 dims a thread) with an online softmax. Bound: the fp32 pipes and the
 // shared-memory loads that feed them (6 16-byte loads for 32 fused multiply-adds).
 // A request's keys are cut into ranges of 64 and more that are joined by a second kernel in order: as many as make, with its row
-// tiles, up to 128 CTAs per kv head (a CTA by itself keeps few loads and sums going: 4 requests of 24 nodes and 1,000 keys on 2 kv
-// heads took 83 us in ranges of 256 keys). The cut
+// tiles, up to 128 CTAs per kv head (a CTA by itself keeps few loads and sums going: 4 requests of 24 nodes and 1,000 keys, 12 heads
+// on 2, took 83 us in ranges of 256 keys; they take 34 to 38, 9 to 10 TFLOP/s; with up to 64 CTAs 40 to 47). The cut
 // depends on the request's own nodes and keys alone, so a node's result does not depend on the batch it was in. Sums run in
 // key order within a row's lane and in a fixed tree across the lanes.
 // A key that a row does not see is left out, not multiplied by zero: what a masked place holds (NaN, infinities) does not matter.

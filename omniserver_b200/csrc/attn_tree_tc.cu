@@ -9,12 +9,17 @@
 // tile's scores are there when a tile's weights are done. A row's exponent offset moves only when its maximum has grown by more
 // than 2^8, and only then do its two threads tell each other their maxima.
 // What bounds it: a tile of keys and values is 32 KB, 0.74 us at a 148th of the memory's rate. Its 64 exponentials a row take 512
-// cycles on a unit that makes 16 a cycle, but the way from tensor memory and back and the waits between the stages take longer
-// (with four softmax warps a tile took 2,090 cycles). So two CTAs share an SM, each with half of its tensor memory and shared memory:
-// while one begins or ends a unit or waits for a product, the other one works.
+// cycles on a unit that makes 16 a cycle, its two products 512 on the tensor cores, but the way from tensor memory and back, the
+// instructions around the exponentials and the waits between the stages take longer (one CTA with four softmax warps: 2,090 cycles a
+// tile). So two CTAs share an SM, each with half of its tensor memory and shared memory: while one begins or ends a unit or waits for
+// a product, the other one works. Each then takes some 1,850 cycles for a tile, the SM half of that, with 57 % of its issue slots taken.
+// Measured (us, with the second kernel): one request of 16 nodes and 2,048 keys, 12 heads on 2, 11.0 (latency: 3 us until the first keys
+// arrive, one or two tiles, 2.5 for the second kernel); 64 requests of 8 nodes and up to 2,100 keys, 28 heads on 4 (206 MB), 50, 4.1
+// TB/s; one of 64 nodes and 32,768 keys, 64 heads on 8 (69 GFLOP), 80 to 83, 840 TFLOP/s.
 //
 // The work is cut evenly: all key tiles of all units (request, kv head, row tile) stand in one line, and every CTA takes an equal
-// piece of it: the end of one unit, some whole ones, the beginning of another. Every CTA finds its piece itself from the
+// piece of it: the end of one unit, some whole ones, the beginning of another. (Where units are few and short, whole ones; see
+// WHOLE_EXTRA.) Every CTA finds its piece itself from the
 // requests' lengths. A unit that was cut leaves its unnormalised fp32 output, maximum and sum in scratch, two places per
 // CTA, laid out [4 dims][row] so that neighbouring threads (rows) write neighbouring 16 bytes straight from tensor memory; a second
 // kernel joins them in order. CTAs of one launch never wait for one another. A single request with several row tiles is the

@@ -14,6 +14,9 @@
 // exp((l - maximum) / T); no two warps wait for each other. `verify_walk_kernel` then needs a few numbers per node to walk the tree;
 // the draw scans one slice of 1,024 words. Only a rejection against a draft's distribution needs its whole row, and the row of
 // logits, once more: then a cluster of CTAs walks the request together, each CTA summing its part of the row.
+// Measured, both kernels: 256 rows of 152,064 words (156 MB) in 8 trees 42.5 us, some 30 of them (5.2 TB/s) the first one, the walk the
+// rest; 32 chains of 6 drafts with draft probabilities (224 of those rows, and some rows of both kinds once more) 48; one chain of 6
+// rows 10.5, of which the walk's chain of loads is 6.
 //
 // Numbers. A word's weight is one fp32 value W = 2^(l c - m c), c = log2(e) / T and m the maximum of its slice, as one fused
 // multiply-add and one exponential (the first kernel has no time for more: at the memory's rate an SM has 22 cycles for 32 words);
@@ -702,9 +705,11 @@ OSB_API int osb_verify_drafts(int* out_tokens, int* out_path, int* out_count, vo
                               draft_probs, T, V, n_slices, max_nodes, max_depth, err);
   };
   if (draft_probs != nullptr && temperature != nullptr) {
-    // a row of draft probabilities is summed by a cluster: of as many CTAs as let every request have its own at once, one per SM
-    int csize = V > 8192 ? MAX_CLUSTER : 1;
-    while (csize > 1 && (long long)S * csize > sms) csize >>= 1;
+    // a row of draft probabilities is summed by a cluster: a CTA per 16,384 words, and as many as let every request have its own at
+    // once, one per SM. Both kernels with 1, 2, 4 and 8 CTAs, us: 8 requests of 7 nodes, 16,384 words 13.6, 14.4, 15.2, 16.7 (the
+    // cluster costs more than the row), 50,000 words 19.8, 18.6, 18.5, 19.4, 152,064 words 45.1, 34.6, 29.3, 27.5
+    int csize = 1;
+    while (csize < MAX_CLUSTER && V >= 2 * csize * 16384 && (long long)S * 2 * csize <= sms) csize <<= 1;
     rc = walk(verify_walk_kernel<true>, osb_allow_smem<verify_walk_kernel<true>>(smem), csize);
   } else {
     rc = walk(verify_walk_kernel<false>, osb_allow_smem<verify_walk_kernel<false>>(smem), 1);
