@@ -561,15 +561,20 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       const int tok = r < seg.rows ? seg.r.q0 + seg.node0 + div_by(r, plan.inv_grp) : -1;   // this row's token, or none
       int lo_row = 0;
       if (plan.window > 0 && tok >= 0) lo_row = seg.r.base + min(max(plan.depth[tok], 0), seg.r.n - 1) - plan.window + 1;
-      float m_run = -INFINITY, l_run = 0.0f;       // the row's exponent offset in use and the sum at it over this half's keys
+      // the row's exponent offset in use (none yet; what is no row has one that nothing exceeds) and the sum at it over this half's keys
+      float m_run = tok >= 0 ? -INFINITY : INFINITY, l_run = 0.0f;
       bool ok = true;
+      // tiles plain0 .. plain1 - 1 are seen whole by every row (tile_masked)
+      const int plain1 = min(seg.r.base, seg.r.kv_len) / TILE_N - seg.tile_begin;
+      const int plain0 = plan.window > 0 ? (max(seg.r.base + seg.r.n - plan.window, 0) + TILE_N - 1) / TILE_N - seg.tile_begin : 0;
       for (int t = 0; t < seg.n_tiles; ++t, ++u) {
         const int key0 = (seg.tile_begin + t) * TILE_N, b = u & 1;
-        const bool masked = tile_masked(seg.r, plan, key0);
+        const bool masked = t < plain0 || t >= plain1;
         unsigned sees = 0u;
         if (masked && tok >= 0) sees = sees32(seg.r, plan, tok, lo_row, key0 + half * 32);
-        if (ok && !mbar_wait(&s_full[b], (uint32_t)(u >> 1) & 1u, vabort)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
+        const uint32_t phase = (uint32_t)(u >> 1) & 1u;
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&s_full[b], phase)))
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&s_full[b], phase, vabort));
         if (!ok) {
           // the other warp of these rows may still have got its scores: it must find this one at the barriers of every tile
           gave_up();
@@ -592,14 +597,13 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
           for (int e = 0; e < 4; ++e)
             mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(v[j + e])), __uint_as_float(v[j + 4 + e]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;  // the scale is positive
-        // the exponent offset in use moves only when the maximum has grown enough (or at the first keys); what lies in rows
-        // that are none moves nothing
-        bool grow = tok >= 0 && (mx > m_run + RESCALE_THRESHOLD || (m_run == -INFINITY && mx > -INFINITY));
+        // the exponent offset in use moves only when the maximum has grown enough, or at the first keys
+        bool grow = mx > m_run + RESCALE_THRESHOLD;
         if (pair_bar_or(qd, grow)) {
           row_max[b][half][r] = mx;
           pair_bar_or(qd, false);
           mx = fmaxf(mx, row_max[b][half ^ 1][r]);
-          grow = tok >= 0 && (mx > m_run + RESCALE_THRESHOLD || (m_run == -INFINITY && mx > -INFINITY));
+          grow = mx > m_run + RESCALE_THRESHOLD;
           const float alpha = (grow && m_run != -INFINITY) ? ex2_approx(m_run - mx) : 1.0f;
           if (grow) m_run = mx;
           if (t > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
