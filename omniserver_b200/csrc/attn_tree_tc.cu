@@ -12,10 +12,10 @@
 // cycles on a unit that makes 16 a cycle, its two products 512 on the tensor cores, but the way from tensor memory and back, the
 // instructions around the exponentials and the waits between the stages take longer (one CTA with four softmax warps: 2,090 cycles a
 // tile). So two CTAs share an SM, each with half of its tensor memory and shared memory: while one begins or ends a unit or waits for
-// a product, the other one works. Each then takes some 1,850 cycles for a tile, the SM half of that, with 57 % of its issue slots taken.
+// a product, the other one works. Each then takes some 1,800 cycles for a tile, the SM half of that, with half of its issue slots taken.
 // Measured (us, with the second kernel): one request of 16 nodes and 2,048 keys, 12 heads on 2, 11.0 (latency: 3 us until the first keys
 // arrive, one or two tiles, 2.5 for the second kernel); 64 requests of 8 nodes and up to 2,100 keys, 28 heads on 4 (206 MB), 50, 4.1
-// TB/s; one of 64 nodes and 32,768 keys, 64 heads on 8 (69 GFLOP), 80 to 83, 840 TFLOP/s.
+// TB/s; one of 64 nodes and 32,768 keys, 64 heads on 8 (69 GFLOP), 79, 870 TFLOP/s (95 in a row of calls, under the power cap).
 //
 // The work is cut evenly: all key tiles of all units (request, kv head, row tile) stand in one line, and every CTA takes an equal
 // piece of it: the end of one unit, some whole ones, the beginning of another. (Where units are few and short, whole ones; see

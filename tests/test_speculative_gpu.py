@@ -1050,6 +1050,8 @@ def test_tree_attention_in_a_cache_of_more_than_2_to_the_32_elements(dtype):
     d = [t.to(DEV) for t in (s.qkv, bt, s.cu, s.lens, s.mask)]
     got = K().tree_attention(d[0], k, v, *d[1:], 4, 2, 128, 128 ** -0.5, None, 9, 209, dtype)
     assert torch.equal(got, want)
+    del k, v
+    torch.cuda.empty_cache()
     K().check_device_errors()
 
 
