@@ -14,8 +14,8 @@
 // exp((l - maximum) / T); no two warps wait for each other. `verify_walk_kernel` then needs a few numbers per node to walk the tree;
 // the draw scans one slice of 1,024 words. Only a rejection against a draft's distribution needs its whole row, and the row of
 // logits, once more: then a cluster of CTAs walks the request together, each CTA summing its part of the row.
-// Measured, both kernels: 256 rows of 152,064 words (156 MB) in 8 trees 42.5 us, some 30 of them (5.2 TB/s) the first one, the walk the
-// rest; 32 chains of 6 drafts with draft probabilities (224 of those rows, and some rows of both kinds once more) 48; one chain of 6
+// Measured, both kernels: 256 rows of 152,064 words (156 MB) in 8 trees 39.3 us, some 27 of them (5.8 TB/s) the first one, the walk the
+// rest; 32 chains of 6 drafts with draft probabilities (224 of those rows, and some rows of both kinds once more) 47; one chain of 6
 // rows 10.5, of which the walk's chain of loads is 6.
 //
 // Numbers. A word's weight is one fp32 value W = 2^(l c - m c), c = log2(e) / T and m the maximum of its slice, as one fused
@@ -35,7 +35,9 @@ constexpr int SLICE = 1024;            // words of a row that a warp of the firs
 constexpr int STAT_THREADS = 128;
 constexpr int STAT_WARPS = STAT_THREADS / 32;
 constexpr int STAT_STAGES = 2;         // slices of a warp in shared memory: the one in hand and the next
-constexpr int STAT_CTAS = 6;           // of the first kernel on an SM: 24 warps of 8 KB
+// Of the first kernel on an SM: 20 warps of 8 KB and 96 registers a thread. (Six leave 80 registers, and fewer loads from shared memory
+// ahead of the arithmetic: 256 rows of 152,064 words 42.5 us with the walk instead of 39.3; four 41.4.)
+constexpr int STAT_CTAS = 5;
 constexpr int PER_LANE = SLICE / 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr float MIN_TEMP = 1e-30f, MAX_TEMP = 1e38f;   // others are taken as these: log2(e) / T is finite and has all its bits
@@ -706,8 +708,8 @@ OSB_API int osb_verify_drafts(int* out_tokens, int* out_path, int* out_count, vo
   };
   if (draft_probs != nullptr && temperature != nullptr) {
     // a row of draft probabilities is summed by a cluster: a CTA per 16,384 words, and as many as let every request have its own at
-    // once, one per SM. Both kernels with 1, 2, 4 and 8 CTAs, us: 8 requests of 7 nodes, 16,384 words 13.6, 14.4, 15.2, 16.7 (the
-    // cluster costs more than the row), 50,000 words 19.8, 18.6, 18.5, 19.4, 152,064 words 45.1, 34.6, 29.3, 27.5
+    // once, one per SM. Both kernels with 1, 2, 4 and 8 CTAs, us: 8 requests of 7 nodes, 16,384 words 13.5, 14.1, 15.1, 16.7 (the
+    // cluster costs more than the row), 50,000 words 19.1, 18.1, 18.4, 19.2, 152,064 words 42.6, 32.6, 28.0, 26.6
     int csize = 1;
     while (csize < MAX_CLUSTER && V >= 2 * csize * 16384 && (long long)S * 2 * csize <= sms) csize <<= 1;
     rc = walk(verify_walk_kernel<true>, osb_allow_smem<verify_walk_kernel<true>>(smem), csize);
