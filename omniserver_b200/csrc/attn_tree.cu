@@ -11,7 +11,7 @@
 // shared-memory loads that feed them (6 16-byte loads for 32 fused multiply-adds).
 // A request's keys are cut into ranges of 64 and more that are joined by a second kernel in order: as many as make, with its row
 // tiles, up to 128 CTAs per kv head (a CTA by itself keeps few loads and sums going: 4 requests of 24 nodes and 1,000 keys, 12 heads
-// on 2, took 83 us in ranges of 256 keys; they take 34, 10 TFLOP/s; with up to 64 CTAs 40 to 47). The cut
+// on 2, took 83 us in ranges of 256 keys; they take 34 to 38, 9 to 10 TFLOP/s; with up to 64 CTAs 40 to 47). The cut
 // depends on the request's own nodes and keys alone, so a node's result does not depend on the batch it was in. Sums run in
 // key order within a row's lane and in a fixed tree across the lanes.
 // A key that a row does not see is left out, not multiplied by zero: what a masked place holds (NaN, infinities) does not matter.
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(NT) attn_tree_kernel(
       s_at[tid] = page < 0 ? -1 : (((long long)page * nkv + kvh) * page_size + key % page_size) * hd;
     }
     __syncthreads();
-#pragma unroll 8      // (a tile's loads at once: 37 us with four)
+#pragma unroll 8      // (a tile's loads at once: 34.5 us for those requests, 36.9 with four)
     for (int i = tid; i < KT * (HDP / 4); i += NT) {
       const int r = i / (HDP / 4), d = (i - r * (HDP / 4)) * 4;
       float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
