@@ -7,7 +7,8 @@
 // r <- max(r - q, 0) / sum (without q: r(x) <- 0, renormalised; r stays as it was if nothing is left). The walk ends where no
 // child is accepted, and the next token is drawn there from r: the smallest index whose running sum passes u times the total,
 // u being the root's random number (the root itself is never tested). Emitted tokens then follow the target's distribution
-// whatever the draft was. Rows with T <= 0 are greedy: p is one at the first largest logit.
+// whatever the draft was. Rows with T <= 0 are greedy: p is one at the first largest logit. A row of which no logit is above -inf accepts nothing, and
+// its next token is 0.
 //
 // Two kernels. `verify_stats_kernel` reads every logit once (what bounds the operator: T x V x 4 bytes): a warp takes 1,024 words of
 // one row in registers, the next 1,024 on their way meanwhile, and leaves their maximum, its first place, and the sum of
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
     if (word < 0 || word >= V) continue;         // no word: it cannot be accepted, and takes nothing away
     bool yes;
     if (greedy) {
-      yes = word == amax[cur];
+      yes = rmx[cur] > -INFINITY && word == amax[cur];      // (a row without logits has no best word)
     } else if (!DENSE) {
       double x = ptok[j];
       for (int k = 0; k < n_rej; ++k)
