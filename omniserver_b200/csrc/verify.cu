@@ -24,7 +24,8 @@
 // m c is rounded, and the slice's factor 2^(m c - m_row c) takes the same rounded numbers, so that all words of
 // a row are off by one common factor and each by some 2^-22 of its own, at random. Sums and comparisons are in 64 bits: what
 // is left of a row behind a random number near 1, or when its largest words were rejected, would not survive 32. A rejected word's
-// weight is the same number that went into its slice's sum, so taking it out leaves the rest exactly.
+// weight is the same number that went into its slice's sum; it is subtracted where that leaves enough of the sum for its digits, and where
+// it does not, what is left is summed again without the rejected words (KEPT).
 #include <cooperative_groups.h>
 
 #include "mma_utils.cuh"
@@ -246,6 +247,10 @@ __global__ void __launch_bounds__(STAT_THREADS, STAT_CTAS) verify_stats_kernel(S
   cp_async_wait<0>();          // nothing of this warp is on its way when its shared memory goes
 }
 
+// A difference of sums is used as long as it is at least this part of the sum that it started from: a sum is right to some 2^-50, so what
+// is left of it to some 2^-26, a sixteenth of what a word's weight is off by.
+constexpr double KEPT = 1.0 / (1 << 24);
+
 constexpr int WALK_THREADS = 512;
 constexpr int WALK_WARPS = WALK_THREADS / 32;
 constexpr int HELD = 5;               // slices a lane keeps in registers (a vocabulary of 163,840 words); more are read again
@@ -271,8 +276,9 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
   WalkSmem& sh = *reinterpret_cast<WalkSmem*>(smem_raw);
   double* ztot = reinterpret_cast<double*>(smem_raw + ((sizeof(WalkSmem) + 15) & ~(size_t)15));   // [max_nodes] a node's total weight
   double* ptok = ztot + max_nodes;                 // [max_nodes] a node's token's weight (DENSE: probability) behind its parent
-  double* rej_w = ptok + max_nodes;                // [max_nodes] without q: the weights of the rejected words
-  float* fac = reinterpret_cast<float*>(rej_w + max_nodes);   // DENSE: [n_slices] probability of a weight of 1, of the node in hand
+  double* psl = ptok + max_nodes;                  // [max_nodes] without q: the weight of the slice that the word is in
+  double* rej_left = psl + max_nodes;              // [max_nodes] without q: what a rejected word left of its slice
+  float* fac = reinterpret_cast<float*>(rej_left + max_nodes);   // DENSE: [n_slices] probability of a weight of 1, of the node in hand
   float* smx = fac + n_slices;                     // DENSE: [n_slices]
   float* rmx = smx + n_slices;                     // [max_nodes] a node's largest logit
   float* qtok = rmx + max_nodes;                   // [max_nodes] q of a node's token
@@ -329,10 +335,13 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
   load_slices(warp);
   auto is_child = [&](int i, int ti, int pi) { return !greedy && pi >= 0 && pi < i && ti >= 0 && ti < V; };
   float tok_l = 0.0f, tok_m = -INFINITY, tok_q = 1.0f;    // of this thread's node: its token's logit, that slice's maximum, q
+  double tok_s = 0.0;                                     // and, without q, its sum
   auto load_token = [&](int i, int ti, int pi) {
     if (!is_child(i, ti, pi)) return;
     tok_l = my_logits[(size_t)pi * V + ti];
-    tok_m = my_stats[(size_t)pi * n_slices + ti / SLICE].mx;
+    const SliceStat& st = my_stats[(size_t)pi * n_slices + ti / SLICE];
+    tok_m = st.mx;
+    if (!DENSE) tok_s = st.sum;
     if (DENSE) tok_q = my_q[(size_t)pi * V + ti];
   };
   load_token(tid, t, p);
@@ -379,10 +388,15 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
   __syncthreads();
   for (int i = tid; i < n; i += WALK_THREADS) {
     const int ti = tok[i], pi = par[i];
-    double x = 0.0;
+    double x = 0.0, in_slice = 0.0;
     if (i != tid) load_token(i, ti, pi);
-    if (is_child(i, ti, pi) && ztot[pi] > 0.0) x = (double)weight_any(tok_l, tok_m, c) * factor(tok_m, rmx[pi], c) * (DENSE ? 1.0 / ztot[pi] : 1.0);
+    if (is_child(i, ti, pi) && ztot[pi] > 0.0) {
+      const double f = factor(tok_m, rmx[pi], c) * (DENSE ? 1.0 / ztot[pi] : 1.0);
+      x = (double)weight_any(tok_l, tok_m, c) * f;
+      if (!DENSE) in_slice = tok_s * f;
+    }
     ptok[i] = x;
+    if (!DENSE) psl[i] = in_slice;
     qtok[i] = is_child(i, ti, pi) ? fmaxf(tok_q, 0.0f) : 1.0f;      // 0 for NaN
   }
   __syncthreads();
@@ -400,6 +414,39 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
   auto after = [&](float x, float q, int k) -> float {
     for (int i = 0; i < k; ++i) x = __fmul_rn(take_out(x, q), rej_inv[i]);
     return x;
+  };
+  // Without q, where differences are not enough: what the first k words of the list leave of slice `sl` of the node in hand, and of its
+  // row. (The whole CTA; the numbers are the same in every thread.)
+  auto cta_sum = [&](double v) -> double {
+    v = warp_sum_d(v);
+    __syncthreads();
+    if (lane == 0) sh.scan[warp] = v;
+    __syncthreads();
+    return warp_sum_d(lane < WALK_WARPS ? sh.scan[lane] : 0.0);
+  };
+  auto sum_slice = [&](int sl, int k) -> double {
+    const float m = my_stats[(size_t)cur * n_slices + sl].mx;
+    const double f = factor(m, rmx[cur], c);
+    double v = 0.0;
+    for (int i = sl * SLICE + tid; i < min(V, (sl + 1) * SLICE); i += WALK_THREADS) {
+      double w = (double)weight_any(my_logits[(size_t)cur * V + i], m, c) * f;
+      for (int r = 0; r < k; ++r)
+        if (rej[r] == i) w = 0.0;
+      v += w;
+    }
+    return cta_sum(v);
+  };
+  // slice sl, whose sum is x
+  auto slice_left = [&](int sl, const SliceStat& x, int k) -> double {
+    for (int r = k - 1; r >= 0; --r)
+      if (rej[r] / SLICE == sl) return rej_left[r];
+    return x.sum * factor(x.mx, rmx[cur], c);
+  };
+  auto sum_row = [&](int k) -> double {
+    const SliceStat* st = my_stats + (size_t)cur * n_slices;
+    double v = 0.0;
+    for (int sl = tid; sl < n_slices; sl += WALK_THREADS) v += slice_left(sl, st[sl], k);
+    return cta_sum(v);
   };
   while (count <= max_depth) {
     // the next child of cur behind the one tested last
@@ -424,16 +471,27 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
         if (rej[k] == word) x = 0.0;             // rejected before: nothing of it is left
       yes = (double)unif[j] * rest < x;
       if (!yes && x > 0.0) {
+        double in_slice = psl[j];
+        for (int k = 0; k < n_rej; ++k)
+          if (rej[k] / SLICE == word / SLICE) in_slice = rej_left[k];
+        in_slice -= x;
         __syncthreads();                          // everyone has read the list
         if (tid == 0) {
           rej[n_rej] = word;
-          rej_w[n_rej] = x;
+          rej_left[n_rej] = in_slice;
         }
         __syncthreads();
+        if (in_slice < psl[j] * KEPT) {
+          in_slice = sum_slice(word / SLICE, n_rej + 1);
+          if (tid == 0) rej_left[n_rej] = in_slice;
+          __syncthreads();
+        }
+        double left = rest - x;
+        if (left < ztot[cur] * KEPT) left = sum_row(n_rej + 1);
         // (where nothing would be left the word stays)
-        if (rest - x > 0.0) {
+        if (left > 0.0) {
           ++n_rej;
-          rest -= x;
+          rest = left;
         }
       }
     } else {
@@ -531,12 +589,7 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
     const SliceStat* st = my_stats + (size_t)cur * n_slices;
     target = (double)unif[0] * rest;
     if (warp == 0) {
-      auto left = [&](int k, const SliceStat& x) -> double {
-        double v = x.sum * factor(x.mx, rmx[cur], c);
-        for (int r = 0; r < n_rej; ++r)
-          if (rej[r] / SLICE == k) v -= rej_w[r];
-        return fmax(v, 0.0);
-      };
+      auto left = [&](int k, const SliceStat& x) -> double { return slice_left(k, x, n_rej); };
       const int per = (n_slices + 31) / 32, k0 = min(lane * per, n_slices), k1 = min(k0 + per, n_slices);
       double held[HELD], v = 0.0;
 #pragma unroll
@@ -672,7 +725,7 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
 }  // namespace
 
 static size_t walk_smem_bytes(int max_nodes, int n_slices) {
-  return ((sizeof(WalkSmem) + 15) & ~(size_t)15) + (size_t)n_slices * 8 + (size_t)max_nodes * (3 * 8 + 9 * 4) + 16;
+  return ((sizeof(WalkSmem) + 15) & ~(size_t)15) + (size_t)n_slices * 8 + (size_t)max_nodes * (4 * 8 + 9 * 4) + 16;
 }
 
 // logits [T, V] fp32; tokens, parents [T] int32 (parents within the request, < 0 for its node 0); cu_q [S + 1]; uniform [T];

@@ -32,3 +32,55 @@ def test_verify_accepts_nothing_on_a_row_without_logits(what, dense):
             if temp is None or temp[s] == 0:
                 assert got[s][2] == 2 and got[s][0][1] == 0
     K().check_device_errors()
+
+
+def uniforms(n, g):
+    return torch.randint(0, 1 << 24, (n,), generator=g).float() / (1 << 24)
+
+
+@pytest.mark.parametrize("temp,others", [(1.0, -math.inf), (0.05, -50.0)])
+def test_verify_slices_of_which_only_rejected_words_had_weight(temp, others):
+    """Two siblings hold all the weight of the first 1,024 words, and the next token's random number is 0: it is the first word with
+    weight behind them. (Their weights are 2^30 and more apart, so that 64 bits do not hold the sum of both.)"""
+    S, V = 64, 5000
+    g = torch.Generator().manual_seed(3)
+    logits = torch.zeros(3 * S, V)
+    rows = torch.full((S, V), others)
+    rows[:, 10] = 0.0
+    rows[:, 500] = (-22.0 - torch.rand(S, generator=g)) * temp
+    rows[:, [3100, 4100]] = (torch.rand(S, 2, generator=g) + 0.1) * temp
+    logits[::3] = rows
+    u = torch.full((3 * S,), 0.99)
+    u[::3] = 0.0
+    for order in ((10, 500), (500, 10)):
+        args = dict(logits=logits, tokens=i32([0, *order] * S), parents=i32([-1, 0, 0] * S), cu_q=i32(list(range(0, 3 * S + 1, 3))), uniform=u)
+        got, want = verify_both(args, 3, 1, torch.full((S,), temp))
+        assert got == want
+        assert all(x == [[3100, -1], [0, -1], 1] for x in got)
+    K().check_device_errors()
+
+
+@pytest.mark.parametrize("apart", [3, 1100])
+@pytest.mark.parametrize("n", [1, 2, 3, 4])
+def test_verify_little_is_left_behind_rejected_words(n, apart):
+    """n siblings, each of which holds all but 2^-22 of what those before it leave, are rejected one after the other (u = 1 - 2^-24): what
+    is left, 2^-88 of the row at the end, is drawn from like any other distribution. The words lie in one slice or in n of them."""
+    S, V = 64, 6000
+    g = torch.Generator().manual_seed(n)
+    words = [700 + apart * i for i in range(n)]
+    rows = torch.randn(S, V, generator=g) * 2.0
+    rows[:, words] = -math.inf
+    rest = torch.logsumexp(rows.double(), -1)
+    for w in reversed(words):
+        rows[:, w] = (rest + 22 * math.log(2.0)).float()
+        rest = torch.logaddexp(rest, rows[:, w].double())
+    logits = torch.zeros(S * (n + 1), V)
+    logits[::n + 1] = rows
+    u = torch.full((S * (n + 1),), 1.0 - 2.0 ** -24)
+    u[::n + 1] = uniforms(S, g)
+    args = dict(logits=logits, tokens=i32(([0] + words) * S), parents=i32(([-1] + [0] * n) * S),
+                cu_q=i32(list(range(0, S * (n + 1) + 1, n + 1))), uniform=u)
+    got, want = verify_both(args, n + 1, 1, torch.ones(S))
+    assert all(x[2] == 1 and x[0][0] not in words for x in want)
+    assert got == want
+    K().check_device_errors()
