@@ -1,0 +1,98 @@
+"""Host code of csrc/ that only shows its faults in rare orders of events, compiled by itself and driven through them on the CPU."""
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from omniserver_b200.ops import library
+
+
+def compiled(tmp_path, name, source, *flags):
+    """The source, which may include csrc's headers, as a shared library."""
+    src, out = tmp_path / f"{name}.cu", tmp_path / f"{name}.so"
+    src.write_text(source)
+    cmd = [library._find_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O1", "-shared", "-Xcompiler", "-fPIC", "-I",
+           library._CSRC, str(src), "-o", str(out), *flags]
+    p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert p.returncode == 0, p.stdout
+    return ctypes.CDLL(str(out))
+
+
+RING = r"""
+#include <random>
+#include <vector>
+#include "attn_tree.cuh"
+
+// The ring of the tree attention's tensor-core kernel: two producers put the tiles K0, K1, V0, K2, V1, .. of each stretch into it, the
+// product S = Q K^T of a tile waits for its keys and for the product P V of the tile before the last, P V for S and its values; a tile
+// leaves its place when its product is complete. Events happen in a random order. Counts the moments at which a tile was under way that
+// the wait before the CTA goes would not have waited for: out[0]; by the last two tiles of each producer alone: out[1].
+template <int STAGES> void run(unsigned seed, int stretches, int most, long long* out) {
+  std::mt19937 rng(seed);
+  std::vector<int> keys, values;          // the ring's tile of each key tile, counted on across stretches
+  for (int k = 0, i0 = 0; k < stretches; ++k) {
+    const int n = 1 + (int)(rng() % most);
+    for (int t = 0; t < n; ++t) {
+      keys.push_back(i0 + (t == 0 ? 0 : 2 * t - 1));
+      values.push_back(i0 + (t + 1 < n ? 2 * t + 2 : 2 * t + 1));
+    }
+    i0 += 2 * n;
+  }
+  const int U = (int)keys.size();
+  enum { NOT_YET, UNDER_WAY, LANDED, USED };
+  std::vector<int> state(2 * U, NOT_YET);
+  attn_tree::UnderWay<STAGES> now;
+  now.clear();
+  int put[2] = {0, 0}, s = 0, s_done = 0, pv = 0, pv_done = 0;
+  std::vector<int> last[2];
+  while (pv_done < U) {
+    const int what = (int)(rng() % 8);
+    if (what < 2) {                                            // a producer
+      if (put[what] == U) continue;
+      const int i = (what == 0 ? keys : values)[put[what]];
+      if (i >= STAGES && state[i - STAGES] != USED) continue;  // waits for `empty`
+      ++put[what];
+      state[i] = UNDER_WAY;
+      now.put(i);
+      last[what].push_back(i);
+    } else if (what < 4) {                                     // a tile lands
+      std::vector<int> flying;
+      for (int i = 0; i < 2 * U; ++i)
+        if (state[i] == UNDER_WAY) flying.push_back(i);
+      if (!flying.empty() && rng() % 4 == 0) state[flying[rng() % flying.size()]] = LANDED;
+    } else if (what == 4) {
+      if (s < U && state[keys[s]] == LANDED && (s < 2 || pv_done > s - 2)) ++s;
+    } else if (what == 5) {
+      if (s_done < s) state[keys[s_done++]] = USED;
+    } else if (what == 6) {
+      if (pv < s_done && state[values[pv]] == LANDED) ++pv;
+    } else if (pv_done < pv) {
+      state[values[pv_done++]] = USED;
+    }
+    for (int i = 0; i < 2 * U; ++i) {
+      if (state[i] != UNDER_WAY) continue;
+      out[0] += now.phase(i % STAGES) != i / STAGES;
+      bool among = false;
+      for (const auto& l : last)
+        for (size_t k = l.size() < 2 ? 0 : l.size() - 2; k < l.size(); ++k) among = among || l[k] == i;
+      out[1] += !among;
+    }
+  }
+}
+extern "C" __attribute__((visibility("default"))) void ring(int stages, unsigned seed, int stretches, int most, long long* out) {
+  if (stages == 4) run<4>(seed, stretches, most, out);
+  else run<8>(seed, stretches, most, out);
+}
+"""
+
+
+def test_a_tree_attention_that_gives_up_waits_for_every_copy_under_way(tmp_path):
+    lib = compiled(tmp_path, "ring", RING)
+    for stages in (4, 8):
+        out = (ctypes.c_longlong * 2)()
+        for seed in range(200):
+            lib.ring(stages, ctypes.c_uint(seed), 1 + seed % 4, 1 + seed % 13, out)
+        assert out[0] == 0, f"{stages} places: a copy under way that nothing waits for"
+        assert out[1] > 0, "the events no longer reach more than two tiles under way"
