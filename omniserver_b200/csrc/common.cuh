@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <mutex>
 #include <type_traits>
 #include <utility>
 
@@ -89,16 +90,22 @@ static inline int osb_num_sms(int* out) {
   *out = n;
   return 0;
 }
+// Lets a kernel have this much dynamic shared memory. What it may have is never made less: a call that needs more may be between here and
+// its launch, in another thread of the host.
 template <auto Kernel> static inline int osb_allow_smem(size_t bytes) {
   static std::atomic<int> allowed[OSB_MAX_DEVICES];
+  static std::mutex one_at_a_time;
   if (bytes <= 48 * 1024) return 0;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  if (dev < OSB_MAX_DEVICES && allowed[dev].load(std::memory_order_relaxed) >= (int)bytes) return 0;
+  if (dev >= OSB_MAX_DEVICES) return OSB_ERR_UNSUPPORTED;
+  if (allowed[dev].load(std::memory_order_acquire) >= (int)bytes) return 0;
+  std::lock_guard<std::mutex> lock(one_at_a_time);
+  if (allowed[dev].load(std::memory_order_relaxed) >= (int)bytes) return 0;
   e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return (int)e;
-  if (dev < OSB_MAX_DEVICES) allowed[dev].store((int)bytes, std::memory_order_relaxed);
+  allowed[dev].store((int)bytes, std::memory_order_release);
   return 0;
 }
 

@@ -96,3 +96,49 @@ def test_a_tree_attention_that_gives_up_waits_for_every_copy_under_way(tmp_path)
             lib.ring(stages, ctypes.c_uint(seed), 1 + seed % 4, 1 + seed % 13, out)
         assert out[0] == 0, f"{stages} places: a copy under way that nothing waits for"
         assert out[1] > 0, "the events no longer reach more than two tiles under way"
+
+
+ALLOW = r"""
+#include <cuda_runtime.h>
+#include <stdlib.h>
+#include <atomic>
+#include <chrono>
+#include <thread>
+
+// The runtime's calls, as far as this test goes: one device, one kernel. Of two calls that set what the kernel may have, the smaller one
+// waits for the larger one to come past it, for half a second at most.
+static std::atomic<int> may_have{0}, larger_set{0}, smaller_in{0};
+template <typename K> static cudaError_t fake_set(K, cudaFuncAttribute, int bytes) {
+  if (bytes == 60000) {
+    smaller_in = 1;
+    for (int i = 0; i < 500 && !larger_set; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+  }
+  may_have = bytes;
+  if (bytes == 100000) larger_set = 1;
+  return cudaSuccess;
+}
+static cudaError_t fake_device(int* dev) {
+  *dev = 0;
+  return cudaSuccess;
+}
+#define cudaFuncSetAttribute fake_set
+#define cudaGetDevice fake_device
+#include "common.cuh"
+
+__global__ void some_kernel() {}
+
+// what the kernel may have when both calls have returned, -1 if one of them failed
+extern "C" __attribute__((visibility("default"))) int allow() {
+  int rc[2] = {0, 0};
+  std::thread small([&] { rc[0] = osb_allow_smem<some_kernel>(60000); });
+  while (!smaller_in) std::this_thread::yield();
+  std::thread large([&] { rc[1] = osb_allow_smem<some_kernel>(100000); });
+  small.join();
+  large.join();
+  return rc[0] || rc[1] ? -1 : (int)may_have;
+}
+"""
+
+
+def test_two_calls_at_once_leave_a_kernel_the_larger_shared_memory(tmp_path):
+    assert compiled(tmp_path, "allow", ALLOW).allow() == 100000
