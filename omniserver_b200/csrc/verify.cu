@@ -739,7 +739,7 @@ OSB_API int osb_verify_drafts(int* out_tokens, int* out_path, int* out_count, vo
   if (S <= 0) return OSB_OK;
   if (V <= 0 || T < 0 || max_nodes < 0 || max_depth < 0) return OSB_ERR_BAD_SHAPE;
   const int n_slices = (V + SLICE - 1) / SLICE;
-  if (max_nodes > 1024 || n_slices > 8192 || (long long)T * n_slices > 2147483647LL || (long long)S * MAX_CLUSTER > 2147483647LL)
+  if (max_nodes > 1024 || max_depth >= 1 << 30 || n_slices > 8192 || (long long)T * n_slices > 2147483647LL || (long long)S * MAX_CLUSTER > 2147483647LL)
     return OSB_ERR_TOO_LARGE;
   int sms = 0;
   int rc = osb_num_sms(&sms);

@@ -152,7 +152,7 @@ class SpeculativeOps:
         _check(cu_q.shape == (S + 1,), "tree_attention: cu_q [S+1]")
         _check(rows == T and 32 * words >= max_q_len, "tree_attention: tree_mask [T, W] with 32 W >= max_q_len")
         _check(hd <= 256, "tree_attention: head sizes up to 256")
-        _check(max_kv_len <= 1 << 30, "tree_attention: up to 2^30 keys per request")
+        _check(max_kv_len <= 1 << 30 and max_q_len <= 1 << 30, "tree_attention: up to 2^30 keys and nodes per request")
         if depth is not None:
             _operands(dev, _I32, "depth", depth)
             _check(depth.shape == (T,), "tree_attention: depth [T]")
@@ -221,7 +221,7 @@ class SpeculativeOps:
         _check(tokens.shape == (T,) and parents.shape == (T,) and uniform.shape == (T,),
                "verify_drafts: tokens, parents and uniform [T]")
         _check(0 <= max_q_len <= self.MAX_TREE_NODES, "verify_drafts: up to 1024 nodes per request")
-        _check(max_depth >= 0, "verify_drafts: max_depth must not be negative")
+        _check(0 <= max_depth < 1 << 30, "verify_drafts: max_depth must not be negative, and below 2^30")
         tp = qp = 0
         if temperature is not None:
             _operands(dev, _F32, "temperature", temperature)

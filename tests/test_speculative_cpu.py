@@ -307,3 +307,8 @@ def test_copy_entry_refuses(src, dst, page_bytes, status):
     a, b = np.array(src, dtype=np.int32), np.array(dst, dtype=np.int32)
     assert library.load().osb_copy_pages(NULL, ctypes.c_longlong(page_bytes), 2, 4, ctypes.c_void_p(a.ctypes.data),
                                          ctypes.c_void_p(b.ctypes.data), len(src), NULL) == status
+
+
+@pytest.mark.parametrize("depth", [1 << 30, (1 << 31) - 1])
+def test_verify_entry_refuses_more_columns_than_it_counts(depth):
+    assert library.load().osb_verify_drafts(*verify_args(depth=depth)) == TOO_LARGE

@@ -84,3 +84,19 @@ def test_verify_little_is_left_behind_rejected_words(n, apart):
     assert all(x[2] == 1 and x[0][0] not in words for x in want)
     assert got == want
     K().check_device_errors()
+
+
+# ------------------------------------------------------------------ bounds of a call
+def test_bounds_that_32_bits_do_not_hold_are_refused():
+    """(The kernels' C entries take these as 32-bit integers: what is beyond would arrive as something else.)"""
+    from omniserver_b200.ops import KernelError
+    z, one = torch.zeros(1, dtype=torch.int32, device=DEV), i32([0, 0]).to(DEV)
+    logits, u = torch.zeros(1, 8, device=DEV), torch.zeros(1, device=DEV)
+    for depth in (1 << 30, (1 << 31) - 1, (1 << 32) + 2):
+        with pytest.raises(KernelError, match="max_depth"):
+            K().verify_drafts(logits, z, z, one, u, 1, depth)
+    k = torch.zeros(1, 1, 16, 64, device=DEV)
+    mask = torch.zeros(1, (1 << 26) + 1, dtype=torch.int32, device=DEV)
+    for most_q, most_kv in (((1 << 31) + 5, 16), (1, (1 << 32) + 16)):
+        with pytest.raises(KernelError, match="2\\^30"):
+            K().tree_attention(torch.zeros(1, 64, device=DEV), k, k, z.view(1, 1), one, z, mask, 1, 1, 64, 1.0, None, most_q, most_kv, torch.float32)
