@@ -6,9 +6,10 @@
 // draft's distribution behind node i (a point mass at x if there is none: u_c < r(x)). A rejection leaves
 // r <- max(r - q, 0) / sum (without q: r(x) <- 0, renormalised; r stays as it was if nothing is left). The walk ends where no
 // child is accepted, and the next token is drawn there from r: the smallest index whose running sum passes u times the total,
-// u being the root's random number (the root itself is never tested). Emitted tokens then follow the target's distribution
-// whatever the draft was. Rows with T <= 0 are greedy: p is one at the first largest logit. A row of which no logit is above -inf accepts nothing, and
-// its next token is 0.
+// u being the root's random number (the root itself is never tested). Emitted tokens then follow the target's distribution:
+// without q whatever the drafts are; with q if siblings were drawn from it independently of one another, the same word twice at times
+// (drawn without putting words back, each would need a q of its own, less the words before it and renormalised). Rows with T <= 0 are
+// greedy: p is one at the first largest logit. A row of which no logit is above -inf accepts nothing, and its next token is 0.
 //
 // Two kernels. `verify_stats_kernel` reads every logit once (what bounds the operator: T x V x 4 bytes): a warp takes 1,024 words of
 // one row in registers, the next 1,024 on their way meanwhile, and leaves their maximum, its first place, and the sum of

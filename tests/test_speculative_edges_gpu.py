@@ -2,11 +2,11 @@
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from plain import speculative as plain
-from test_speculative_gpu import DEV, K, drafts, i32, verify_both
+from test_speculative_gpu import BF16, DEV, F32, K, Step, check, drafts, i32, runs_on_tensor_cores, verify_both
 
 pytestmark = pytest.mark.gpu
 
@@ -83,6 +83,39 @@ def test_verify_little_is_left_behind_rejected_words(n, apart):
     got, want = verify_both(args, n + 1, 1, torch.ones(S))
     assert all(x[2] == 1 and x[0][0] not in words for x in want)
     assert got == want
+    K().check_device_errors()
+
+
+def test_verify_siblings_drawn_independently_leave_the_targets_distribution():
+    """Three siblings and, below the first, another: drawn independently of one another from their parent's row of draft probabilities, or,
+    without draft probabilities, the same different words every time. The first two emitted tokens are distributed like the target's:
+    20,000 walks, a count's standard deviation is at most sqrt(N / 4): 6 of them."""
+    N, V, n = 20000, 8, 5
+    g = torch.Generator().manual_seed(4)
+    target = torch.randn(V, V, generator=g)                  # by the word before: node c's row is that of its token
+    draft = torch.softmax(torch.randn(V, V, generator=g), -1)
+    p = torch.softmax(target.double(), -1)
+    for dense in (False, True):
+        tokens = torch.zeros(N, n, dtype=torch.long)         # the root's token is 0
+        if dense:
+            tokens[:, 1:4] = torch.multinomial(draft[0], 3 * N, replacement=True, generator=g).view(N, 3)
+            tokens[:, 4] = torch.multinomial(draft[tokens[:, 1]], 1, generator=g)[:, 0]
+        else:
+            tokens[:, 1:] = torch.tensor([5, 2, 7, 1])
+        u = uniforms(N * n, g)
+        flat = tokens.view(-1)
+        new, path, count = K().verify_drafts(target[flat].to(DEV), flat.to(torch.int32).to(DEV), i32([-1, 0, 0, 0, 1] * N).to(DEV),
+                                             torch.arange(0, n * N + 1, n, dtype=torch.int32).to(DEV), u.to(DEV), n, 2, torch.ones(N, device=DEV),
+                                             draft[flat].to(DEV) if dense else None)
+        new, count = new.cpu().long(), count.cpu()
+        first = torch.bincount(new[:, 0], minlength=V).double()
+        assert ((first - N * p[0]).abs() <= 6 * math.sqrt(N / 4)).all()
+        # where there is a second token in this step, it follows the first like the target says
+        for w in range(V):
+            second = torch.bincount(new[(new[:, 0] == w) & (count > 1), 1], minlength=V).double()
+            m = float(second.sum())
+            assert ((second - m * p[w]).abs() <= 6 * math.sqrt(m / 4) + 1e-9).all()
+        assert len(count.unique()) == 3
     K().check_device_errors()
 
 
