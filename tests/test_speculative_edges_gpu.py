@@ -119,6 +119,109 @@ def test_verify_siblings_drawn_independently_leave_the_targets_distribution():
     K().check_device_errors()
 
 
+@pytest.mark.parametrize("dense", [False, True])
+@pytest.mark.parametrize("V", [170001, 330000])
+def test_verify_rows_of_more_slices_than_a_lane_holds(V, dense):
+    """Most of the weight, the drawn words and the drafted ones lie behind the first 160 slices of 1,024 words, or in the last ones."""
+    for q_lens, tail in (([5], 3000), ([3, 4], 1000), ([4, 3, 3], V - 163840)):
+        args, q = drafts(q_lens, V, seed=V + tail, branch=2, peak=3.0, dense=dense)
+        args["logits"][:, -tail:] += 9.0
+        if dense:
+            q[:, -tail:] *= 1000.0
+            q /= q.sum(-1, keepdim=True)
+        for j in range(1, sum(q_lens)):
+            if j not in args["cu_q"].tolist():
+                s = sum(j >= x for x in args["cu_q"][1:].tolist())
+                row = int(args["cu_q"][s]) + int(args["parents"][j])
+                args["tokens"][j] = int(args["logits"][row, -tail:].topk(3).indices[j % 3]) + V - tail
+        seen = 0
+        for temp in (None, torch.full((len(q_lens),), 0.9)):
+            got, want = verify_both(args, max(q_lens), 3, temp, q)
+            assert got == want
+            seen += sum(x[0][x[2] - 1] >= V - tail for x in got)
+        assert seen > 0
+    K().check_device_errors()
+
+
+@pytest.mark.parametrize("reqs", [1, 9])
+@pytest.mark.parametrize("V", [33000, 40001, 70000, 99999])
+def test_verify_walks_by_two_and_four_ctas(V, reqs):
+    accepted = 0
+    for seed in range(3):
+        args, q = drafts([4 + (i + seed) % 3 for i in range(reqs)], V, seed=seed + reqs, branch=3, peak=3.0, dense=True)
+        got, want = verify_both(args, 6, 4, torch.full((reqs,), 0.8), q)
+        assert got == want
+        accepted += sum(x[2] - 1 for x in got)
+    assert accepted > 0 or reqs == 1      # (three trees of one request may accept nothing)
+    K().check_device_errors()
+
+
+# ------------------------------------------------------------------ attention
+def window_step(q_lens, bases, nh, nkv, hd, window, dtype, seed):
+    step = Step(q_lens, bases, nh, nkv, hd, 16, dtype, seed=seed)
+    for s, b in enumerate(bases):                 # pages that every row's window has passed were given back
+        for pi in range(max(0, b - window + 1) // 16):
+            step.bt[s, pi] = -1
+    return step
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q_lens,bases,nh,nkv,hd,window", [
+    ([24], [3000], 12, 2, 128, 1500), ([70], [2049], 8, 2, 64, 640), ([40], [1000], 28, 4, 128, 5000),      # row tiles abreast
+    ([8, 5, 12], [3000, 2000, 2500], 12, 2, 128, 1100), ([30, 1, 9], [4000, 700, 1300], 28, 4, 64, 2000),   # units cut, one row tile and two
+    ([64, 33], [1700, 900], 7, 1, 128, 1001), ([6, 20], [2100, 2500], 2, 2, 64, 2047)])
+def test_tree_attention_windows_of_units_that_are_cut(q_lens, bases, nh, nkv, hd, window, dtype):
+    step = window_step(q_lens, bases, nh, nkv, hd, window, dtype, seed=window)
+    check(step, step.got(window), *step.want(window), runs_on_tensor_cores(step))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_tree_attention_batches_cut_at_many_places(hd, which):
+    rng = np.random.default_rng(8)
+    bases = (rng.integers(1500, 2200, 64).tolist(), rng.integers(0, 300, 200).tolist(), [20000, 5, 700, 64, 3000])[which]
+    step = Step([int(x) for x in rng.integers(1, 9, len(bases))], bases, 28, 4, hd, 64, BF16, seed=8)
+    check(step, step.got(), *step.want(), True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q_lens,bases", [([3], [40]), ([5, 1, 9], [300, 20, 1100]), ([17, 2], [2000, 129])])
+def test_tree_attention_with_bounds_above_what_is_there(q_lens, bases, dtype):
+    """As a captured step passes them: the most nodes and keys that there may be."""
+    step = Step(q_lens, bases, 12, 2, 128, 32, dtype, seed=5)
+    wide = torch.full((len(q_lens), 300), -1, dtype=torch.int32)
+    wide[:, :step.bt.shape[1]] = step.bt
+    mask = torch.zeros(step.mask.shape[0], 4, dtype=torch.int32)
+    mask[:, :step.mask.shape[1]] = step.mask
+    for most_q, most_kv in ((32, 2100), (100, 9600), (128, 1 << 20)):
+        out = K().tree_attention(step.qkv.to(DEV), step.k.to(DEV), step.v.to(DEV), wide.to(DEV), step.cu.to(DEV), step.lens.to(DEV), mask.to(DEV),
+                                 12, 2, 128, 128 ** -0.5, None, most_q, most_kv, dtype)
+        check(step, out, *step.want(), runs_on_tensor_cores(step))
+
+
+class Rows:
+    """Some requests of a step, for `check`."""
+
+    def __init__(self, step, n):
+        self.q_lens, self.lens, self.hd = step.q_lens[:n], step.lens[:n], step.hd
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tree_attention_computes_the_requests_beside_a_reported_one(dtype):
+    from omniserver_b200.ops import KernelError
+    s = Step([5, 9], [30, 140], 4, 2, 64, 16, dtype, seed=2)
+    want, spread, weight = s.want()
+    d = [t.to(DEV) for t in (s.qkv, s.k, s.v, s.bt, s.cu, s.lens, s.mask)]
+    cases = [(d, 8, 149), (d, 9, 148)]                                       # too many nodes, too many keys
+    cases += [(d[:4] + [i32(cu).to(DEV)] + d[5:], 9, 149) for cu in ([0, 5, 15], [0, 5, 2])]   # tokens that are not there
+    cases += [(d[:5] + [i32([35, 4]).to(DEV)] + d[6:], 9, 149)]              # fewer keys than nodes
+    for args, most_q, most_kv in cases:
+        got = K().tree_attention(*args, 4, 2, 64, 0.125, None, most_q, most_kv, dtype)
+        with pytest.raises(KernelError, match="more nodes or keys"):
+            K().check_device_errors()
+        check(Rows(s, 1), got[:5], want[:5], spread[:5], weight, dtype == BF16)
+
+
 # ------------------------------------------------------------------ bounds of a call
 def test_bounds_that_32_bits_do_not_hold_are_refused():
     """(The kernels' C entries take these as 32-bit integers: what is beyond would arrive as something else.)"""
