@@ -31,8 +31,8 @@
 // would still reach the row through the tensor core: in such tiles the values that are not finite are replaced by zeros in shared
 // memory, and if there were any, the rows that do see them get them added at the end, from the cache.
 //
-// All mbarrier waits are bounded; on a time-out the CTA records a code in *err, waits (bounded too) for its copies and products under
-// way, frees its tensor memory and returns.
+// All mbarrier waits are bounded; on a time-out the CTA records a code in *err, frees its tensor memory and returns. Each warp that issues
+// copies or products waits (bounded too) until they are done before it leaves, whoever gave up, and before the tensor memory goes.
 #include "attn_tree.cuh"
 #include "tc_utils.cuh"
 
@@ -239,6 +239,9 @@ __device__ __forceinline__ bool pair_bar_or(int quarter, bool v) {
   return r != 0;
 }
 
+// Barrier of the two warps that fill the ring.
+__device__ __forceinline__ void producers_bar() { asm volatile("bar.sync 7, 64;" ::: "memory"); }
+
 template <int HD>
 struct Layout {
   static constexpr int NA = HD / 64;                  // 64-element atoms along the head dimension
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   __shared__ uint64_t q_full, staged_out, full[STAGES], empty[STAGES], s_full[2], p_full[2], pv_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ UnderWay<STAGES> under_way;
+  __shared__ int ring_end[2][STAGES];     // the tile that each producer put into a place of the ring last
   __shared__ int found_bad[3];            // by the number of the CTA's stretch modulo 3: values that are not finite were taken out of a V tile
   __shared__ int scan[NUM_THREADS / 32];
   __shared__ int start_s, start_p;        // the request in which this CTA's piece begins, where its units begin
@@ -284,7 +287,6 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   if (lane == 0 && warp < 3) prefetch_tensormap(warp == 0 ? &map_k : warp == 1 ? &map_q : &map_v);
   if (tid == 0) {
     abort_flag = 0;
-    under_way.clear();
     found_bad[0] = found_bad[1] = found_bad[2] = 0;
     start_s = 0;
     mbar_init(&q_full, 1);
@@ -404,6 +406,7 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
     const bool keys = warp == 0;
     const CUtensorMap* map = keys ? &map_k : &map_v;
     int i0 = 0;             // tiles that were put into the ring before this stretch, by both
+    LastPut<STAGES> last_put;               // of this warp's tiles; lane k has the ring's place k
     for (; !*vabort && walk.next(plan, seg); i0 += 2 * seg.n_tiles) {
       const int p_last = seg.r.kv_len - 1;
       auto page_of = [&](int t) -> int {      // of this lane's box of tile t
@@ -445,10 +448,17 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
               tma_load_4d(to + a * KV_ATOM + b * box_rows * 128, map, &full[st], a * 64, (row0 + b * box_rows) & (ps - 1), seg.kvh, pg);
           }
         }
-        if (lane == 0) under_way.put(i);
+        last_put.put(lane, i);
         page = next_page;
         next_page = after_next;
       }
+    }
+    // when neither puts anything more, they wait until what was put into each place last has landed
+    if (lane < STAGES) ring_end[keys ? 0 : 1][lane] = last_put.tile;
+    __syncwarp();
+    producers_bar();
+    const int i = lane < STAGES ? max(ring_end[0][lane], ring_end[1][lane]) : -1;
+    for (uint32_t w = 0; i >= 0 && w < WAIT_LIMIT && !mbar_try_wait(&full[lane], (uint32_t)(i / STAGES) & 1u); ++w) {
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ loads Q, issues S = Q K^T
@@ -500,10 +510,11 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
         if (!*vabort) atomicExch(err, 112);
         *vabort = 1;
       }
+      for (uint32_t w = 0; q_issued > 0 && w < WAIT_LIMIT && !mbar_try_wait(&q_full, (uint32_t)(q_issued - 1) & 1u); ++w) {
+      }
     }
-    if (lane == 0) {
-      under_way.q = q_issued;
-      under_way.s = u;
+    // the last product completes, and so have those before it
+    for (uint32_t w = 0; u > 0 && w < WAIT_LIMIT && !mbar_try_wait(&s_full[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u); ++w) {
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------------ issuer of O += P V
@@ -534,7 +545,8 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
       if (!*vabort) atomicExch(err, 112);
       *vabort = 1;
     }
-    if (lane == 0) under_way.pv = u;
+    for (uint32_t w = 0; u > 0 && w < WAIT_LIMIT && !mbar_try_wait(&pv_done[(u - 1) & 1], (uint32_t)((u - 1) >> 1) & 1u); ++w) {
+    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
@@ -780,19 +792,6 @@ __global__ void __launch_bounds__(NUM_THREADS, CTAS_PER_SM) attn_tree_tc_kernel(
   fence_before();
   __syncthreads();
   if (warp == 1) {
-    if (*vabort) {
-      // a lane waits for a place of the ring, the next three for the last load of Q and the last product of either kind
-      uint64_t* bar = lane < STAGES ? &full[lane] : &q_full;
-      int phase = lane < STAGES ? under_way.phase(lane) : lane == STAGES ? under_way.q - 1 : -1;
-      if (lane == STAGES + 1 || lane == STAGES + 2) {
-        const int last = (lane == STAGES + 1 ? under_way.s : under_way.pv) - 1;
-        bar = lane == STAGES + 1 ? &s_full[last & 1] : &pv_done[last & 1];
-        phase = last >> 1;       // (-1 where there was none)
-      }
-      for (uint32_t w = 0; phase >= 0 && w < WAIT_LIMIT && !mbar_try_wait(bar, (uint32_t)phase & 1u); ++w) {
-      }
-      __syncwarp();
-    }
     fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }

@@ -27,8 +27,9 @@ RING = r"""
 
 // The ring of the tree attention's tensor-core kernel: two producers put the tiles K0, K1, V0, K2, V1, .. of each stretch into it, the
 // product S = Q K^T of a tile waits for its keys and for the product P V of the tile before the last, P V for S and its values; a tile
-// leaves its place when its product is complete. Events happen in a random order. Counts the moments at which a tile was under way that
-// the wait before the CTA goes would not have waited for: out[0]; by the last two tiles of each producer alone: out[1].
+// leaves its place when its product is complete. Events happen in a random order. Counts the tiles, at every moment, that are under way and
+// that the producers, if they stopped now, would not wait for: out[0]; if each waited for the last two that it put: out[1]. And the places
+// whose wait would not end when everything has landed, since the barrier is in a later phase of the same parity: out[2].
 template <int STAGES> void run(unsigned seed, int stretches, int most, long long* out) {
   std::mt19937 rng(seed);
   std::vector<int> keys, values;          // the ring's tile of each key tile, counted on across stretches
@@ -43,10 +44,10 @@ template <int STAGES> void run(unsigned seed, int stretches, int most, long long
   const int U = (int)keys.size();
   enum { NOT_YET, UNDER_WAY, LANDED, USED };
   std::vector<int> state(2 * U, NOT_YET);
-  attn_tree::UnderWay<STAGES> now;
-  now.clear();
+  attn_tree::LastPut<STAGES> now[2][STAGES];
   int put[2] = {0, 0}, s = 0, s_done = 0, pv = 0, pv_done = 0;
   std::vector<int> last[2];
+  int phases[STAGES] = {};                // of each place's barrier that have begun
   while (pv_done < U) {
     const int what = (int)(rng() % 8);
     if (what < 2) {                                            // a producer
@@ -55,7 +56,8 @@ template <int STAGES> void run(unsigned seed, int stretches, int most, long long
       if (i >= STAGES && state[i - STAGES] != USED) continue;  // waits for `empty`
       ++put[what];
       state[i] = UNDER_WAY;
-      now.put(i);
+      ++phases[i % STAGES];
+      for (int k = 0; k < STAGES; ++k) now[what][k].put(k, i);
       last[what].push_back(i);
     } else if (what < 4) {                                     // a tile lands
       std::vector<int> flying;
@@ -71,9 +73,14 @@ template <int STAGES> void run(unsigned seed, int stretches, int most, long long
     } else if (pv_done < pv) {
       state[values[pv_done++]] = USED;
     }
+    int noted[STAGES];
+    for (int k = 0; k < STAGES; ++k) {
+      noted[k] = now[0][k].tile > now[1][k].tile ? now[0][k].tile : now[1][k].tile;
+      out[2] += noted[k] >= 0 && ((noted[k] / STAGES) & 1) == (phases[k] & 1);
+    }
     for (int i = 0; i < 2 * U; ++i) {
       if (state[i] != UNDER_WAY) continue;
-      out[0] += now.phase(i % STAGES) != i / STAGES;
+      out[0] += noted[i % STAGES] != i;
       bool among = false;
       for (const auto& l : last)
         for (size_t k = l.size() < 2 ? 0 : l.size() - 2; k < l.size(); ++k) among = among || l[k] == i;
@@ -91,10 +98,11 @@ extern "C" __attribute__((visibility("default"))) void ring(int stages, unsigned
 def test_a_tree_attention_that_gives_up_waits_for_every_copy_under_way(tmp_path):
     lib = compiled(tmp_path, "ring", RING)
     for stages in (4, 8):
-        out = (ctypes.c_longlong * 2)()
+        out = (ctypes.c_longlong * 3)()
         for seed in range(200):
             lib.ring(stages, ctypes.c_uint(seed), 1 + seed % 4, 1 + seed % 13, out)
         assert out[0] == 0, f"{stages} places: a copy under way that nothing waits for"
+        assert out[2] == 0, f"{stages} places: a wait that does not end"
         assert out[1] > 0, "the events no longer reach more than two tiles under way"
 
 
