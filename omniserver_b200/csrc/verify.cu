@@ -467,14 +467,13 @@ __global__ void __launch_bounds__(WALK_THREADS, 1) verify_walk_kernel(
     if (greedy) {
       yes = rmx[cur] > -INFINITY && word == amax[cur];      // (a row without logits has no best word)
     } else if (!DENSE) {
-      double x = ptok[j];
-      for (int k = 0; k < n_rej; ++k)
+      double x = ptok[j], in_slice = psl[j];
+      for (int k = 0; k < n_rej; ++k) {
         if (rej[k] == word) x = 0.0;             // rejected before: nothing of it is left
+        if (rej[k] / SLICE == word / SLICE) in_slice = rej_left[k];
+      }
       yes = (double)unif[j] * rest < x;
       if (!yes && x > 0.0) {
-        double in_slice = psl[j];
-        for (int k = 0; k < n_rej; ++k)
-          if (rej[k] / SLICE == word / SLICE) in_slice = rej_left[k];
         in_slice -= x;
         __syncthreads();                          // everyone has read the list
         if (tid == 0) {
