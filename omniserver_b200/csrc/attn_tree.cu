@@ -7,8 +7,11 @@
 //
 // The query rows of a request and kv head are its nodes times the group's heads (row = node x group + head). A CTA takes 32 rows
 // and one range of keys in tiles of 32: keys and values pass through shared memory as fp32 once for all rows, scores and outputs
-// are register tiles (4 rows x 2 keys, 4 rows x HD / 16 dims a thread) with an online softmax. Bound: the fp32 pipes and the
-// shared-memory loads that feed them (6 16-byte loads for 32 fused multiply-adds).
+// are register tiles (4 rows x 2 keys, 4 rows x HD / 16 dims a thread) with an online softmax.
+// What bounds it at the sizes of a step of drafted tokens is latency: a CTA has a few tiles, loads one, meets three barriers and sums, with
+// nothing of the next tile under way, and three CTAs share an SM (134 registers a thread at 128 dims; the 64-dim forms keep 12 to 20 bytes in
+// local memory). 4 requests of 24 nodes and 1,000 keys, 12 heads on 2, by counters: 16 % of an SM's warps, the fp32 pipe 25 % and the
+// load pipe 16 % busy, a third of a warp's time between instructions spent on loads from memory.
 // A request's keys are cut into ranges of 64 and more that are joined by a second kernel in order: as many as make, with its row
 // tiles, up to 128 CTAs per kv head (a CTA by itself keeps few loads and sums going: 4 requests of 24 nodes and 1,000 keys, 12 heads
 // on 2, took 83 us in ranges of 256 keys; they take 34 to 38, 9 to 10 TFLOP/s; with up to 64 CTAs 40 to 47). The cut

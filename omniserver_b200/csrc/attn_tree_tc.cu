@@ -15,7 +15,7 @@
 // a product, the other one works. Each then takes some 1,800 cycles for a tile, the SM half of that, with half of its issue slots taken.
 // Measured (us, with the second kernel): one request of 16 nodes and 2,048 keys, 12 heads on 2, 11.0 (latency: 3 us until the first keys
 // arrive, one or two tiles, 2.5 for the second kernel); 64 requests of 8 nodes and up to 2,100 keys, 28 heads on 4 (206 MB), 50, 4.1
-// TB/s; one of 64 nodes and 32,768 keys, 64 heads on 8 (69 GFLOP), 79, 870 TFLOP/s (95 in a row of calls, under the power cap).
+// TB/s; one of 64 nodes and 32,768 keys, 64 heads on 8 (69 GFLOP), 95 in a row of calls, under the power cap: 720 TFLOP/s (by itself 79).
 //
 // The work is cut evenly: all key tiles of all units (request, kv head, row tile) stand in one line, and every CTA takes an equal
 // piece of it: the end of one unit, some whole ones, the beginning of another. (Where units are few and short, whole ones; see
@@ -936,8 +936,8 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   if (rc == 0 && z.cuts) {
     const int units = plan.S * plan.nkv * plan.m_tiles;
     // warps for so many dims each and so many sharing the pieces of a row: as many as make about one wave. Both kernels with each
-    // of the four, in this order, us: one request of 2,048 keys on 2 kv heads 13.7, 14.7, 15.7, 20.3; 8 ragged ones of up to 4,096
-    // on 4 kv heads 41.8, 31.0, 29.5, 31.0; 64 of 2,100 79.7, 56.3, 51.8, 50.7
+    // of the four, in this order, us: one request of 2,048 keys on 2 kv heads 10.9, 12.2, 14.4, 22.7; 8 ragged ones of up to 4,096
+    // on 4 kv heads 40.9, 30.3, 28.7, 30.3; 64 of 2,100 78.2, 55.2, 51.0, 49.6
     const long long groups = (long long)units * z.row_blocks, wave = 12LL * z.ctas;
     auto join = [&](auto k, int dims, int warps) {
       const int per_unit = z.row_blocks * (HD / dims), per_cta = 8 / warps;

@@ -4,8 +4,8 @@
 // of their request (base: the request's committed tokens) and have to lie at base + i, in every layer, for keys, values and
 // every head. A path ascends, so path[i] >= i and a token never moves onto one that has yet to move if they move in order:
 // a thread owns one piece of 16 bytes of one head's row and takes it along the whole path, up to eight tokens in flight, so no
-// order between threads is needed. Bound: one round trip to memory (a few tokens of 4 to 16 KB a layer): 3.2 us for one request in 28
-// layers of 2 heads, 5.6 for 64 requests in 28 of 4 (10.9 MB).
+// order between threads is needed. Bound: four loads in a chain (counts and offsets, the path, page numbers, tokens; a few of 4 to 16 KB a
+// layer): 3.1 us for one request in 28 layers of 2 heads, 5.6 for 64 requests in 28 of 4 (10.9 MB).
 //
 // `copy_pages_kernel`: whole pages, e.g. the last, partly filled page of a request that is forked. A page of one layer's keys or
 // values is contiguous; a CTA copies 16 KB of it with 16-byte loads, four in flight per thread. Bound: the copy rate of the

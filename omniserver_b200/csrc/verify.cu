@@ -16,9 +16,9 @@
 // exp((l - maximum) / T); no two warps wait for each other. `verify_walk_kernel` then needs a few numbers per node to walk the tree;
 // the draw scans one slice of 1,024 words. Only a rejection against a draft's distribution needs its whole row, and the row of
 // logits, once more: then a cluster of CTAs walks the request together, each CTA summing its part of the row.
-// Measured, both kernels: 256 rows of 152,064 words (156 MB) in 8 trees 39.3 us, some 27 of them (5.8 TB/s) the first one, the walk the
+// Measured, both kernels: 256 rows of 152,064 words (156 MB) in 8 trees 39.8 us, some 27 of them (5.8 TB/s) the first one, the walk the
 // rest; 32 chains of 6 drafts with draft probabilities (224 of those rows, and some rows of both kinds once more) 47; one chain of 6
-// rows 10.5, of which the walk's chain of loads is 6.
+// rows 10.3, of which the walk's chain of loads is 6.
 //
 // Numbers. A word's weight is one fp32 value W = 2^(l c - m c), c = log2(e) / T and m the maximum of its slice, as one fused
 // multiply-add and one exponential (the first kernel has no time for more: at the memory's rate an SM has 22 cycles for 32 words);
