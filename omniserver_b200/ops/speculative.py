@@ -205,7 +205,8 @@ class SpeculativeOps:
         renormalised, or without ``draft_probs`` (drafts that are certain of their token) the word itself. ``draft_probs`` [T, V]
         fp32: row i is the distribution that node i's children were drawn from, each independently of the others (with replacement; the new
         tokens follow the target's distribution only then, without ``draft_probs`` always); negative and NaN entries count as 0. NaN logits
-        count as -inf; where no logit of a row is above -inf nothing is accepted and the next token is 0. ``max_q_len``: at least the
+        count as -inf; where no logit of a row is above -inf nothing is accepted and the next token is 0. Words of 2^-126 of the likeliest
+        one's probability and less may count as having none. ``max_q_len``: at least the
         most nodes of a request; what a larger one has beyond it is not looked at, nor a request whose tokens are outside
         ``logits`` (count 0), and ``check_device_errors`` reports them.
 

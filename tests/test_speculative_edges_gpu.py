@@ -86,6 +86,25 @@ def test_verify_little_is_left_behind_rejected_words(n, apart):
     K().check_device_errors()
 
 
+@pytest.mark.parametrize("slices", [(7, 9), (7, 1500)])
+def test_verify_draws_words_down_to_the_end_of_32_bits(slices):
+    """A random number of 0 draws the first word that has weight: one of 2^-120 of the largest has, one of 2^-160 may have (a slice's own
+    largest word counts for it), one of -inf has not. Before a rejection and behind one (the first of two words of a half each goes), with and
+    without draft probabilities."""
+    V = 4000
+    light, heavy = slices
+    row = torch.full((V,), -math.inf)
+    row[5], row[light], row[[heavy, 3000]] = -160 * math.log(2.0), -120 * math.log(2.0), 0.0
+    logits = torch.stack([row] * 3)
+    q = torch.zeros(3, V)
+    q[:, heavy] = 1.0
+    args = dict(logits=logits, tokens=i32([0, 0, heavy]), parents=i32([-1, -1, 0]), cu_q=i32([0, 1, 3]), uniform=torch.tensor([0.0, 0.0, 0.9]))
+    for dense in (False, True):
+        got, _ = verify_both(args, 2, 1, torch.ones(2), q if dense else None)
+        assert all(x[0][0] in (5, light) and x[1:] == [[0, -1], 1] for x in got)
+    K().check_device_errors()
+
+
 def test_verify_siblings_drawn_independently_leave_the_targets_distribution():
     """Three siblings and, below the first, another: drawn independently of one another from their parent's row of draft probabilities, or,
     without draft probabilities, the same different words every time. The first two emitted tokens are distributed like the target's:
